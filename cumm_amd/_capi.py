@@ -74,6 +74,36 @@ class OrderSide(C.Structure):
                 ("by_position", C.c_void_p), ("by_position_reversed", C.c_void_p)]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("out_dtype", C.c_int32), ("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32),
+                ("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+                ("out", C.c_void_p), ("pre_act", C.c_void_p), ("ld_x", C.c_int64), ("ld_weight", C.c_int64),
+                ("ld_residual", C.c_int64), ("ld_out", C.c_int64), ("ld_pre_act", C.c_int64), ("x_scale", C.c_void_p),
+                ("weight_scale", C.c_void_p), ("act_type", C.c_int32), ("act_alpha", C.c_float), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class LinearGradArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("m", C.c_int64), ("n", C.c_int32), ("k", C.c_int32), ("grad_out", C.c_void_p),
+                ("pre_act", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("ld_grad_out", C.c_int64),
+                ("ld_pre_act", C.c_int64), ("ld_x", C.c_int64), ("ld_weight", C.c_int64), ("grad_x", C.c_void_p),
+                ("grad_weight", C.c_void_p), ("grad_bias", C.c_void_p), ("act_type", C.c_int32), ("act_alpha", C.c_float),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class RmsNormArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("k", C.c_int32), ("m", C.c_int64), ("x", C.c_void_p), ("residual", C.c_void_p),
+                ("weight", C.c_void_p), ("ld_x", C.c_int64), ("ld_residual", C.c_int64), ("out", C.c_void_p), ("total", C.c_void_p),
+                ("codes", C.c_void_p), ("scale", C.c_void_p), ("inv_rms", C.c_void_p), ("eps", C.c_float)]
+
+
+class RmsNormGradArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("k", C.c_int32), ("m", C.c_int64), ("total", C.c_void_p), ("weight", C.c_void_p),
+                ("grad_out", C.c_void_p), ("grad_total", C.c_void_p), ("ld_total", C.c_int64), ("ld_grad_out", C.c_int64),
+                ("ld_grad_total", C.c_int64), ("inv_rms", C.c_void_p), ("grad_x", C.c_void_p), ("grad_weight", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # every symbol include/cumm_hip.h declares: name -> (restype, argtypes)
 _VP, _PVP = C.c_void_p, C.POINTER(C.c_void_p)
 SYMBOLS = {
@@ -150,6 +180,13 @@ SYMBOLS = {
     "cumm_hip_column_sum": (C.c_int, [_VP, _VP, C.c_int64, C.c_int, C.c_int, _VP, C.c_size_t, _VP]),
     "cumm_hip_gate_sums": (C.c_int, [C.POINTER(GateSums), C.c_int, _VP]),
     "cumm_hip_relu_backward_sums": (C.c_int, [_VP, _VP, _VP, _VP, C.c_int64, C.c_int, C.c_int, _VP, C.c_size_t, _VP]),
+    "cumm_hip_linear_workspace": (C.c_int64, [C.POINTER(LinearArgs)]),
+    "cumm_hip_linear": (C.c_int, [C.POINTER(LinearArgs), _VP]),
+    "cumm_hip_linear_backward_workspace": (C.c_int64, [C.POINTER(LinearGradArgs)]),
+    "cumm_hip_linear_backward": (C.c_int, [C.POINTER(LinearGradArgs), _VP]),
+    "cumm_hip_rms_norm": (C.c_int, [C.POINTER(RmsNormArgs), _VP]),
+    "cumm_hip_rms_norm_backward_workspace": (C.c_int64, [C.POINTER(RmsNormGradArgs)]),
+    "cumm_hip_rms_norm_backward": (C.c_int, [C.POINTER(RmsNormGradArgs), _VP]),
     "cumm_hip_gather_rows": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, C.c_size_t, _VP]),
     "cumm_hip_scatter_add_rows": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, C.c_int, C.c_int, _VP]),
 }

@@ -1842,3 +1842,7 @@ int cumm_hip_copy_kernel(void *dst, const void *src, size_t bytes, void *stream)
 }
 
 }  // extern "C"
+
+namespace cummhip {
+int layer_error(int code, const char *what) { return fail(code, "%s", what); }
+}  // namespace cummhip

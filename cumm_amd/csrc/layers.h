@@ -1,0 +1,71 @@
+// Host side of the row-wise layers: products with an epilogue (linear_inst.hip) and norms (rownorm_inst.hip)
+#pragma once
+#include "linear.h"
+
+namespace cummhip {
+
+// the calling thread's last error (cumm_hip_last_error); returns code
+int layer_error(int code, const char *what);
+
+// ---- products
+enum LinearLayout { kResult = 0, kGradInput = 1, kGradWeight = 2 };      // (XT, YT) = (0, 0), (1, 0), (1, 1)
+// Which kernel, and into how many slices the contraction is cut
+struct LinearPlan {
+  int tile;      // kTile*
+  int slices;
+};
+enum LinearTile { kTileFew = 0, kTile64 = 1, kTile128 = 2, kTile128Deep = 3, kTile256 = 4 };
+// k in units of two bytes
+LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k);
+// bytes of the slices' sums (0 = one slice)
+inline int64_t linear_partial_bytes(const LinearPlan &plan, int64_t m, int n) {
+  return plan.slices > 1 ? (int64_t)plan.slices * m * ((n + 7) / 8 * 8) * 4 : 0;
+}
+hipError_t launch_linear_f16(LinearLayout layout, const LinearPlan &plan, const LinearParams &p, hipStream_t s);
+hipError_t launch_linear_bf16(LinearLayout layout, const LinearPlan &plan, const LinearParams &p, hipStream_t s);
+// 8-bit operands, output f16 or bf16 (layout kResult)
+hipError_t launch_linear_s8(bool bf16, const LinearPlan &plan, const LinearParams &p, hipStream_t s);
+// rows x cols elements of 1 or 2 bytes to rows of to_ld bytes (a multiple of 16), zeros behind them
+hipError_t launch_linear_repack(void *to, const void *from, int64_t rows, int64_t cols, int64_t ld, int64_t to_ld, int elem_bytes, hipStream_t s);
+
+struct LinearGateParams {
+  const void *grad;        // [rows, n]
+  const void *pre;         // [rows, n] what the activation got, NULL = it is none
+  void *dz;                // [rows, ldz], NULL = sums only
+  int64_t ldg, ldp, ldz;   // elements; ldz: those of a row that are written, n rounded up to 8
+  int64_t dz_pitch;
+  float *partial;          // [blocks, pitch], NULL = no sums
+  int64_t rows, rows_per_block;
+  int32_t n, pitch, shift, act;
+  float slope;
+};
+void linear_gate_shape(int64_t rows, int n, int *shift, int *strips, int *blocks, int64_t *per);
+hipError_t launch_linear_gate(LinearGateParams p, int64_t dz_pitch, void *grad_bias, bool bf16, hipStream_t s);
+// two-byte elements (a kernel: memset nodes of captured graphs have given wrong results on replays)
+hipError_t launch_rows_zero(void *dst, int64_t elements, hipStream_t s);
+
+// ---- norms
+struct NormParams {
+  const void *x, *residual;      // rows of k elements; residual may be NULL
+  const void *weight;            // [k]; NULL = no norm
+  void *out, *total;             // [rows, k]
+  int8_t *codes;                 // [rows, k] instead of out
+  float *scale, *inv;            // [rows]; inv may be NULL
+  int64_t rows, ldx, ldr;
+  int32_t k;
+  float eps;
+};
+hipError_t launch_norm(const NormParams &p, int dtype, hipStream_t s);
+struct NormGradParams {
+  const void *h, *weight, *grad, *grad_total;      // grad or grad_total may be NULL: zeros
+  const float *inv;
+  void *grad_in;           // [rows, k], may be NULL
+  void *grad_weight;       // [k]
+  float *partial;          // [blocks, pitch]; NULL = no grad_weight
+  int64_t rows, ldh, ldg, ldt;
+  int32_t k, pitch, blocks;
+};
+int norm_backward_blocks(int64_t rows, int k);
+hipError_t launch_norm_backward(const NormGradParams &p, bool bf16, hipStream_t s);
+
+}  // namespace cummhip

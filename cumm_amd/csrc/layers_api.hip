@@ -1,0 +1,357 @@
+// C entry points of the row-wise layers: argument checks, the layout of the workspace, launches.
+#include "../../include/cumm_hip.h"
+
+#include "layers.h"
+
+using namespace cummhip;
+
+namespace {
+
+int bad(const char *what) { return layer_error(CUMM_HIP_EINVAL, what); }
+int launched(hipError_t e) { return e == hipSuccess ? CUMM_HIP_OK : layer_error(CUMM_HIP_ERUNTIME, hipGetErrorString(e)); }
+
+bool two_byte(int dt) { return dt == CUMM_HIP_F16 || dt == CUMM_HIP_BF16; }
+bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool on(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+constexpr int64_t kRowBytes = (int64_t)8 << 20;      // 256 rows of a tile lie within 2^31 bytes
+constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int kMaxWhole = 131071;                    // 8-bit operands: k * 128 * 128 < 2^31
+
+// Pieces of the workspace in the order they are asked for: their sum, and, once there is a base, their places
+struct Workspace {
+  char *base;
+  int64_t used = 0;
+  void *take(int64_t bytes) {
+    void *at = base ? base + used : nullptr;
+    used += up(bytes, 256);
+    return at;
+  }
+};
+
+// A matrix operand as the products read it: its own rows where they lie on 16-byte borders and are whole 16-byte pieces long,
+// else a copy of them (lines of 128 bytes apart) in the workspace
+struct Operand {
+  const void *from;
+  int64_t rows, cols, ld;      // elements
+  int bytes;                   // of one
+  void *copy = nullptr;
+  bool direct() const { return on16(from) && ld * bytes % 16 == 0 && cols * bytes % 16 == 0; }
+  int64_t pitch() const { return direct() ? ld * bytes : up(cols * bytes, 128); }
+  const void *at() const { return direct() ? from : copy; }
+  void place(Workspace &w) {
+    if (!direct()) copy = w.take(rows * pitch());
+  }
+  hipError_t fill(hipStream_t s) const { return direct() ? hipSuccess : launch_linear_repack(copy, from, rows, cols, ld, pitch(), bytes, s); }
+};
+
+bool tiles_fit(int64_t m, int64_t n) { return (m + 63) / 64 * ((n + 63) / 64) <= 0x7fffffff; }
+
+const char *linear_checked(const CummHipLinearArgs &a) {
+  const bool s8 = a.dtype == CUMM_HIP_S8;
+  if (!s8 && !two_byte(a.dtype)) return "linear: operands are f16, bf16 or s8";
+  if (s8 ? !two_byte(a.out_dtype) : a.out_dtype != a.dtype) return "linear: the output is f16 or bf16, that of the operands unless they are s8";
+  if (a.m < 0 || a.m > kMaxRows || a.n < 1 || a.k < 1) return "linear: m, n and k must not be empty (m may be 0) or exceed int32 range";
+  const int size = s8 ? 1 : 2;
+  if (a.ld_x < a.k || a.ld_weight < a.k || a.ld_out < a.n || (a.residual && a.ld_residual < a.n) || (a.pre_act && a.ld_pre_act < a.n))
+    return "linear: rows overlap (a pitch is smaller than its row)";
+  if (a.ld_x * size >= kRowBytes || a.ld_weight * size >= kRowBytes || up((int64_t)a.k * size, 128) >= kRowBytes) return "linear: rows of 8 MiB and more are not taken";
+  if (s8 && a.k > kMaxWhole) return "linear: sums of more than 131071 products of 8 bits may exceed int32 range";
+  if (!tiles_fit(a.m, a.n)) return "linear: too many outputs for one launch";
+  if (a.act_type < 0 || a.act_type > CUMM_HIP_ACT_GELU_TANH) return "linear: unknown activation";
+  if (a.m == 0) return nullptr;
+  if (!a.x || !a.weight || !a.out) return "linear: x, weight and out must not be null";
+  if (s8 && (!a.x_scale || !a.weight_scale)) return "linear: 8-bit operands need the scales of their rows";
+  if (!on(a.x, size) || !on(a.weight, size) || !on(a.out, 2) || !on(a.residual, 2) || !on(a.pre_act, 2) || !on(a.bias, s8 ? 4 : 2) ||
+      (s8 && (!on(a.x_scale, 4) || !on(a.weight_scale, 4))))
+    return "linear: a pointer is not aligned to its elements";
+  return nullptr;
+}
+
+struct LinearCall {
+  Operand x, weight;
+  LinearPlan plan;
+  int64_t k2;      // k in units of two bytes, as the copies have it
+  void *partial;
+  LinearCall(const CummHipLinearArgs &a, Workspace &w) {
+    const int size = a.dtype == CUMM_HIP_S8 ? 1 : 2;
+    x = {a.x, a.m, a.k, a.ld_x, size};
+    weight = {a.weight, a.n, a.k, a.ld_weight, size};
+    x.place(w);
+    weight.place(w);
+    k2 = up((int64_t)a.k * size, 16) / 2;
+    plan = linear_plan(kResult, a.m, a.n, k2);
+    partial = plan.slices > 1 ? w.take(linear_partial_bytes(plan, a.m, a.n)) : nullptr;
+  }
+};
+
+hipError_t launch_two_byte(int dtype, LinearLayout layout, const LinearPlan &plan, const LinearParams &p, hipStream_t s) {
+  return dtype == CUMM_HIP_BF16 ? launch_linear_bf16(layout, plan, p, s) : launch_linear_f16(layout, plan, p, s);
+}
+
+const char *linear_grad_checked(const CummHipLinearGradArgs &a) {
+  if (!two_byte(a.dtype)) return "linear backward: f16 or bf16";
+  if (a.m < 0 || a.m > kMaxRows || a.n < 1 || a.k < 1) return "linear backward: m, n and k must not be empty (m may be 0) or exceed int32 range";
+  if (a.act_type < 0 || a.act_type > CUMM_HIP_ACT_GELU_TANH) return "linear backward: unknown activation";
+  if (a.ld_grad_out < a.n || (a.pre_act && a.ld_pre_act < a.n) || (a.x && a.ld_x < a.k) || (a.weight && a.ld_weight < a.k))
+    return "linear backward: rows overlap (a pitch is smaller than its row)";
+  const int64_t most = kRowBytes / 2;
+  if (a.ld_grad_out >= most || a.ld_x >= most || a.ld_weight >= most || up(a.n, 64) >= most || up(a.k, 64) >= most)
+    return "linear backward: rows of 8 MiB and more are not taken";
+  if (!tiles_fit(a.m, a.k) || !tiles_fit(a.n, a.k)) return "linear backward: too many outputs for one launch";
+  if (a.m == 0) return nullptr;
+  if (a.grad_x && !a.weight) return "linear backward: the gradient of x needs the weight";
+  if (a.grad_weight && !a.x) return "linear backward: the gradient of the weight needs x";
+  if (!a.grad_out) return "linear backward: grad_out must not be null";
+  if (a.act_type != CUMM_HIP_ACT_NONE && !a.pre_act) return "linear backward: the activation's argument (pre_act) is missing";
+  for (const void *p : {a.grad_out, a.pre_act, a.x, a.weight, (const void *)a.grad_x, (const void *)a.grad_weight, (const void *)a.grad_bias})
+    if (!on(p, 2)) return "linear backward: a pointer is not aligned to its elements";
+  return nullptr;
+}
+
+struct LinearGradCall {
+  Operand x, weight;
+  LinearGateParams gate = {};
+  bool gated;              // a launch that writes dz, or the bias sums, or both
+  const void *dz;
+  int64_t ldz;             // elements
+  LinearPlan plan_x = {0, 1}, plan_w = {0, 1};
+  void *partial_x = nullptr, *partial_w = nullptr;
+  LinearGradCall(const CummHipLinearGradArgs &a, Workspace &w) {
+    const bool act = a.act_type != CUMM_HIP_ACT_NONE, products = a.grad_x || a.grad_weight;
+    const Operand g = {a.grad_out, a.m, a.n, a.ld_grad_out, 2};
+    const bool write = products && (act || !g.direct());
+    gated = write || a.grad_bias;
+    dz = a.grad_out;
+    ldz = a.ld_grad_out;
+    gate.grad = a.grad_out;
+    gate.pre = act ? a.pre_act : nullptr;
+    gate.ldg = a.ld_grad_out;
+    gate.ldp = a.ld_pre_act;
+    gate.rows = a.m;
+    gate.n = a.n;
+    gate.act = a.act_type;
+    gate.slope = a.act_alpha;
+    gate.pitch = (int)up(a.n, 16);
+    if (write) {
+      ldz = up(a.n, a.n >= 64 ? 64 : 8);
+      dz = gate.dz = w.take(a.m * ldz * 2);
+      gate.ldz = up(a.n, 8);      // (what is written of a row; its pitch is ldz)
+    }
+    if (a.grad_bias) {
+      int shift, strips, blocks;
+      int64_t per;
+      linear_gate_shape(a.m, a.n, &shift, &strips, &blocks, &per);
+      gate.partial = reinterpret_cast<float *>(w.take((int64_t)blocks * gate.pitch * 4));
+    }
+    if (a.grad_x) {
+      weight = {a.weight, a.n, a.k, a.ld_weight, 2};
+      weight.place(w);
+      plan_x = linear_plan(kGradInput, a.m, a.k, a.n);
+      if (plan_x.slices > 1) partial_x = w.take(linear_partial_bytes(plan_x, a.m, a.k));
+    }
+    if (a.grad_weight) {
+      x = {a.x, a.m, a.k, a.ld_x, 2};
+      x.place(w);
+      plan_w = linear_plan(kGradWeight, a.n, a.k, a.m);
+      if (plan_w.slices > 1) partial_w = w.take(linear_partial_bytes(plan_w, a.n, a.k));
+    }
+  }
+};
+
+const char *norm_checked(const CummHipRmsNormArgs &a) {
+  const bool norm = a.weight != nullptr;
+  if (!two_byte(a.dtype) && !(a.dtype == CUMM_HIP_F32 && !norm && !a.out)) return "rms norm: f16 or bf16 (f32 for rows in 8 bits without a norm)";
+  if (a.m < 0 || a.m > kMaxRows || a.k < 1) return "rms norm: rows must not be empty, their number must not exceed int32 range";
+  if (a.ld_x < a.k || (a.residual && a.ld_residual < a.k)) return "rms norm: rows overlap (a pitch is smaller than its row)";
+  if (norm && !(a.eps > 0.0f)) return "rms norm: eps must be positive";
+  if (!norm && (a.residual || a.total || a.inv_rms)) return "rms norm: no residual, sum or statistics without a norm";
+  if ((a.residual != nullptr) != (a.total != nullptr) && a.m > 0) return "rms norm: the sum is written where there is a residual, and only there";
+  if (a.m == 0) return nullptr;
+  if (!a.x || (a.out != nullptr) == (a.codes != nullptr)) return "rms norm: x, and either out or codes, must not be null";
+  if (!norm && !a.codes) return "rms norm: a norm needs its weight";
+  if ((a.codes != nullptr) != (a.scale != nullptr)) return "rms norm: a scale per row goes with 8-bit rows";
+  const int size = a.dtype == CUMM_HIP_F32 ? 4 : 2;
+  if (!on(a.x, size) || !on(a.residual, 2) || !on(a.weight, 2) || !on(a.out, 2) || !on(a.total, 2) || !on(a.scale, 4) || !on(a.inv_rms, 4))
+    return "rms norm: a pointer is not aligned to its elements";
+  return nullptr;
+}
+
+const char *norm_grad_checked(const CummHipRmsNormGradArgs &a) {
+  if (!two_byte(a.dtype)) return "rms norm backward: f16 or bf16";
+  if (a.m < 0 || a.m > kMaxRows || a.k < 1) return "rms norm backward: rows must not be empty, their number must not exceed int32 range";
+  if (a.ld_total < a.k || (a.grad_out && a.ld_grad_out < a.k) || (a.grad_total && a.ld_grad_total < a.k))
+    return "rms norm backward: rows overlap (a pitch is smaller than its row)";
+  if (a.m == 0) return nullptr;
+  if (!a.total || !a.weight || !a.inv_rms) return "rms norm backward: total, weight and inv_rms must not be null";
+  for (const void *p : {a.total, a.weight, a.grad_out, a.grad_total, (const void *)a.grad_x, (const void *)a.grad_weight})
+    if (!on(p, 2)) return "rms norm backward: a pointer is not aligned to its elements";
+  if (!on(a.inv_rms, 4)) return "rms norm backward: a pointer is not aligned to its elements";
+  return nullptr;
+}
+
+const char *workspace_checked(const void *workspace, size_t bytes, int64_t need) {
+  if (need == 0) return nullptr;
+  if (!workspace || (int64_t)bytes < need) return "the workspace is smaller than cumm_hip_*_workspace says";
+  return on(workspace, 256) ? nullptr : "the workspace must be 256-byte aligned";
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t cumm_hip_linear_workspace(const CummHipLinearArgs *a) {
+  if (!a || linear_checked(*a)) return -1;
+  if (a->m == 0) return 0;
+  Workspace w = {nullptr};
+  LinearCall call(*a, w);
+  return w.used;
+}
+
+int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
+  if (!a) return bad("linear: null arguments");
+  if (const char *e = linear_checked(*a)) return bad(e);
+  if (a->m == 0) return CUMM_HIP_OK;
+  Workspace w = {reinterpret_cast<char *>(a->workspace)};
+  const LinearCall call(*a, w);
+  if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipError_t e = call.x.fill(s);
+  if (e == hipSuccess) e = call.weight.fill(s);
+  if (e != hipSuccess) return launched(e);
+  LinearParams p = {};
+  p.X = call.weight.at();
+  p.Y = call.x.at();
+  p.ldx = call.weight.pitch();
+  p.ldy = call.x.pitch();
+  p.m = a->m;
+  p.n = a->n;
+  p.k = call.k2;
+  p.out = a->out;
+  p.ldo = a->ld_out;
+  p.bias = a->bias;
+  p.residual = a->residual;
+  p.ldr = a->ld_residual;
+  p.pre = a->pre_act;
+  p.ldp = a->ld_pre_act;
+  p.y_scale = a->x_scale;
+  p.x_scale = a->weight_scale;
+  p.act = a->act_type;
+  p.slope = a->act_alpha;
+  p.partial = call.partial;
+  p.slices = call.plan.slices;
+  if (a->dtype == CUMM_HIP_S8) return launched(launch_linear_s8(a->out_dtype == CUMM_HIP_BF16, call.plan, p, s));
+  return launched(launch_two_byte(a->dtype, kResult, call.plan, p, s));
+}
+
+int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *a) {
+  if (!a || linear_grad_checked(*a)) return -1;
+  if (a->m == 0) return 0;
+  Workspace w = {nullptr};
+  LinearGradCall call(*a, w);
+  return w.used;
+}
+
+int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
+  if (!a) return bad("linear backward: null arguments");
+  if (const char *e = linear_grad_checked(*a)) return bad(e);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a->m == 0) {
+    hipError_t e = a->grad_weight ? launch_rows_zero(a->grad_weight, (int64_t)a->n * a->k, s) : hipSuccess;
+    if (e == hipSuccess && a->grad_bias) e = launch_rows_zero(a->grad_bias, a->n, s);
+    return launched(e);
+  }
+  Workspace w = {reinterpret_cast<char *>(a->workspace)};
+  const LinearGradCall call(*a, w);
+  if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
+  const bool bf16 = a->dtype == CUMM_HIP_BF16;
+  hipError_t e = call.gated ? launch_linear_gate(call.gate, call.ldz, a->grad_bias, bf16, s) : hipSuccess;
+  if (e == hipSuccess && a->grad_x) {
+    e = call.weight.fill(s);
+    LinearParams p = {};
+    p.Y = call.dz;
+    p.ldy = call.ldz * 2;
+    p.X = call.weight.at();
+    p.ldx = call.weight.pitch();
+    p.m = a->m;
+    p.n = a->k;
+    p.k = a->n;
+    p.out = a->grad_x;
+    p.ldo = a->k;
+    p.partial = call.partial_x;
+    p.slices = call.plan_x.slices;
+    if (e == hipSuccess) e = launch_two_byte(a->dtype, kGradInput, call.plan_x, p, s);
+  }
+  if (e == hipSuccess && a->grad_weight) {
+    e = call.x.fill(s);
+    LinearParams p = {};
+    p.Y = call.dz;
+    p.ldy = call.ldz * 2;
+    p.X = call.x.at();
+    p.ldx = call.x.pitch();
+    p.m = a->n;
+    p.n = a->k;
+    p.k = a->m;
+    p.out = a->grad_weight;
+    p.ldo = a->k;
+    p.partial = call.partial_w;
+    p.slices = call.plan_w.slices;
+    if (e == hipSuccess) e = launch_two_byte(a->dtype, kGradWeight, call.plan_w, p, s);
+  }
+  return launched(e);
+}
+
+int cumm_hip_rms_norm(const CummHipRmsNormArgs *a, void *stream) {
+  if (!a) return bad("rms norm: null arguments");
+  if (const char *e = norm_checked(*a)) return bad(e);
+  if (a->m == 0) return CUMM_HIP_OK;
+  NormParams p = {};
+  p.x = a->x;
+  p.residual = a->residual;
+  p.weight = a->weight;
+  p.out = a->out;
+  p.total = a->total;
+  p.codes = a->codes;
+  p.scale = a->scale;
+  p.inv = a->inv_rms;
+  p.rows = a->m;
+  p.ldx = a->ld_x;
+  p.ldr = a->ld_residual;
+  p.k = a->k;
+  p.eps = a->eps;
+  return launched(launch_norm(p, a->dtype, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int64_t cumm_hip_rms_norm_backward_workspace(const CummHipRmsNormGradArgs *a) {
+  if (!a || norm_grad_checked(*a)) return -1;
+  return a->m == 0 || !a->grad_weight ? 0 : up((int64_t)norm_backward_blocks(a->m, a->k) * up(a->k, 16) * 4, 256);
+}
+
+int cumm_hip_rms_norm_backward(const CummHipRmsNormGradArgs *a, void *stream) {
+  if (!a) return bad("rms norm backward: null arguments");
+  if (const char *e = norm_grad_checked(*a)) return bad(e);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a->m == 0) return launched(a->grad_weight ? launch_rows_zero(a->grad_weight, a->k, s) : hipSuccess);
+  if (!a->grad_x && !a->grad_weight) return CUMM_HIP_OK;
+  if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, cumm_hip_rms_norm_backward_workspace(a))) return bad(e);
+  NormGradParams p = {};
+  p.h = a->total;
+  p.weight = a->weight;
+  p.grad = a->grad_out;
+  p.grad_total = a->grad_total;
+  p.inv = a->inv_rms;
+  p.grad_in = a->grad_x;
+  p.grad_weight = a->grad_weight;
+  p.partial = a->grad_weight ? reinterpret_cast<float *>(a->workspace) : nullptr;
+  p.rows = a->m;
+  p.ldh = a->ld_total;
+  p.ldg = a->ld_grad_out;
+  p.ldt = a->ld_grad_total;
+  p.k = a->k;
+  p.pitch = (int)up(a->k, 16);
+  p.blocks = norm_backward_blocks(a->m, a->k);
+  return launched(launch_norm_backward(p, a->dtype == CUMM_HIP_BF16, s));
+}
+
+}  // extern "C"

@@ -1,0 +1,614 @@
+// Matrix product of rows with a weight, bias, activation and residual in its epilogue,
+//   out[m][n] = act( sum_k x[m][k] w[n][k] + bias[n] ) + residual[m][n],
+// and the two products of its backward pass, on matrix cores:
+//   D[m][n] = sum_k Y[m][k] X[n][k]      X, Y contiguous along k, or along their rows (XT, YT)
+//     result            Y = x,             X = w
+//     grad_x            Y = dz [m][n],     X = w  read along its rows (the contraction is over n)
+//     grad_weight       Y = dz, X = x, both along their rows (the contraction is over m)
+// Operands lie in LDS as densegemm_lds.h has them (DenseOperand: permuted 16-byte chunks, direct-to-LDS
+// loads, hand-counted waits).  What is different here:
+//   * addresses are 64 bits: a tile's descriptor begins at its own first row and moves by a step's bytes, so
+//     that no operand has a size limit; offsets inside a tile's step stay below 2^31 bytes (checked on the host);
+//   * 8-bit operands are pairs of bytes to the copies and the LDS layout, only the products know them;
+//   * the contraction can be cut into slices (grid.y), whose 32-bit sums a second kernel adds up in order;
+//   * the epilogue below.
+#pragma once
+#include "densegemm_lds.h"
+#include "rows.h"
+
+namespace cummhip {
+
+enum LinearAct { kActNone = 0, kActRelu = 1, kActSigmoid = 2, kActLeakyRelu = 3, kActSilu = 4, kActGelu = 5, kActGeluTanh = 6 };
+
+struct LinearParams {
+  const void *X, *Y;       // operand indexed by n, by m
+  int64_t ldx, ldy;        // bytes between rows (XT, YT: between k slices)
+  int64_t m;
+  int32_t n;
+  int64_t k;               // of two bytes each: elements, pairs of 8-bit ones
+  void *out;
+  int64_t ldo;             // elements, as ldr and ldp
+  const void *bias;        // [n] in the output's type, f32 with 8-bit operands; NULL = none
+  const void *residual;    // [m, n] or NULL
+  int64_t ldr;
+  void *pre;               // [m, n]: what the activation gets, for the backward pass; NULL = not wanted
+  int64_t ldp;
+  const float *y_scale, *x_scale;   // 8-bit operands: [m], [n]
+  int32_t act;
+  float slope;
+  void *partial;           // slices > 1: [slices][m][n8] 32-bit sums, n8 = n rounded up to 8
+  int32_t slices;
+};
+
+// ---- the epilogue: values v[8] are consecutive columns n .. n + 7 of a row
+
+// log2(e), and of 2 sqrt(2 / pi) (z + 0.044715 z^3): the tanh form of the gelu is z times the logistic function of that
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kGeluA = 2.30220819813f, kGeluB = 0.10294324038f;      // kLog2e * 2 sqrt(2/pi), the same * 0.044715
+
+__device__ __forceinline__ float logistic_of_exponent(float t) {      // 1 / (1 + 2^t)
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+}
+// Half of erfc(|z| / sqrt 2), the smaller tail of the normal distribution: Abramowitz and Stegun 7.1.26 (error of erf below
+// 1.5e-7), and e^(-z^2 / 2) beside it
+__device__ __forceinline__ float normal_tail(float z, float *e) {
+  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+  float poly = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  poly = __builtin_fmaf(poly, t, 1.421413741f);
+  poly = __builtin_fmaf(poly, t, -0.284496736f);
+  poly = __builtin_fmaf(poly, t, 0.254829592f);
+  *e = __builtin_amdgcn_exp2f(x * x * -kLog2e);
+  return 0.5f * poly * t * *e;
+}
+
+// The activation is uniform: one dispatch for a lane's values.  NaN stays NaN.
+template <int N>
+__device__ __forceinline__ void linear_act(float (&v)[N], int act, float slope) {
+  switch (act) {
+  case kActRelu:
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+    break;
+  case kActLeakyRelu:
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? v[i] * slope : v[i];
+    break;
+  case kActSigmoid:
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = logistic_of_exponent(-kLog2e * v[i]);
+    break;
+  case kActSilu:
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= logistic_of_exponent(-kLog2e * v[i]);
+    break;
+  case kActGeluTanh:
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= logistic_of_exponent(-v[i] * __builtin_fmaf(kGeluB, v[i] * v[i], kGeluA));
+    break;
+  case kActGelu:
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float e;
+      const float tail = normal_tail(v[i], &e);
+      v[i] *= v[i] < 0.0f ? tail : 1.0f - tail;
+    }
+    break;
+  default: break;
+  }
+}
+
+// the derivative of the activation where its argument is z
+__device__ __forceinline__ float linear_act_slope(float z, int act, float slope) {
+  switch (act) {
+  case kActRelu: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  case kActLeakyRelu: return z > 0.0f ? 1.0f : (z != z ? z : slope);
+  case kActSigmoid: {
+    const float p = logistic_of_exponent(-kLog2e * z);
+    return p * (1.0f - p);
+  }
+  case kActSilu: {
+    const float p = logistic_of_exponent(-kLog2e * z);
+    return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+  }
+  case kActGeluTanh: {
+    const float p = logistic_of_exponent(-z * __builtin_fmaf(kGeluB, z * z, kGeluA));
+    // z p(u(z)): p + z p (1 - p) u', u' = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2); beyond |z| = 16, where p is 0 or 1, the
+    // cubic term would be infinite times zero
+    const float zc = __builtin_fminf(__builtin_fmaxf(z, -16.0f), 16.0f);
+    const float du = __builtin_fmaf(0.21406572f * zc, zc, 1.59576912f);
+    return __builtin_fmaf(zc * p * (1.0f - p), du, p);
+  }
+  case kActGelu: {
+    float e;
+    const float tail = normal_tail(z, &e);
+    const float zc = __builtin_fminf(__builtin_fmaxf(z, -16.0f), 16.0f);
+    return (z < 0.0f ? tail : 1.0f - tail) + zc * e * 0.39894228040143268f;
+  }
+  default: return 1.0f;
+  }
+}
+
+// Bias of columns n .. n + 7, and what the accumulators are multiplied by (8-bit operands)
+template <class OUT, bool S8>
+__device__ __forceinline__ void linear_columns(const LinearParams &p, int n, float (&bias)[8], float (&scale)[8]) {
+  const int count = p.n - n;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bias[e] = 0.0f;
+  if constexpr (S8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) scale[e] = e < count ? p.x_scale[n + e] : 0.0f;
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bias[e] = e < count ? reinterpret_cast<const float *>(p.bias)[n + e] : 0.0f;
+    }
+  } else {
+    if (p.bias != nullptr && count > 0) {
+      Piece<OUT> b;
+      b.load(p.bias, n, count);
+      b.values(bias);
+    }
+  }
+}
+
+// One row's eight columns out of sums: the whole epilogue
+template <class OUT, bool S8, bool NT>
+__device__ __forceinline__ void linear_finish8(const LinearParams &p, int64_t m, int n, float (&v)[8], const float (&bias)[8], const float (&scale)[8]) {
+  const int count = p.n - n;
+  Piece<OUT> piece, add;
+  add.raw = v4i{0, 0, 0, 0};
+  if (p.residual != nullptr) add.load(p.residual, m * p.ldr + n, count);
+  const float row = S8 ? p.y_scale[m] : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = S8 ? __builtin_fmaf(v[e] * row, scale[e], bias[e]) : v[e] + bias[e];
+  if (p.pre != nullptr) {
+    piece.round(v);
+    piece.template store<NT>(p.pre, m * p.ldp + n, count);
+  }
+  linear_act(v, p.act, p.slope);
+  float r[8];
+  add.values(r);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += r[e];
+  piece.round(v);
+  piece.template store<NT>(p.out, m * p.ldo + n, count);
+}
+
+// A wave's accumulators, RBW x NBW blocks of 16 x 16 from row m_wave, column n_wave on.  Lane (q, i) holds four columns
+// of each block, of row i.  They go through the wave's share of LDS (BYTES of it, CHUNK row blocks at a time) and come
+// back as eight consecutive columns a lane: whole lines of 64 or 128 bytes per row and store, and a loop over rows instead
+// of an epilogue written out for every accumulator, which needs more registers than the large tile leaves.  Rows are
+// [row][16 or 8 units of four columns], units permuted by the row: neither side meets a bank twice.
+template <class OUT, bool S8, int RBW, int NBW, bool XT, bool NT, int BYTES, class AccV>
+__device__ __forceinline__ void linear_epilogue(const LinearParams &p, const AccV (&acc)[RBW][NBW], int64_t m_wave, int n_wave, int lane, char *lds) {
+  constexpr int UNITS = NBW * 4, PIECES = NBW * 2, ROWS = 64 / PIECES;      // ROWS at a time
+  constexpr int FIT = BYTES / (NBW * 1024), CHUNK = FIT < RBW ? FIT : RBW;
+  static_assert((NBW == 2 || NBW == 4) && CHUNK >= 1 && RBW % CHUNK == 0, "row blocks of a chunk");
+  const int i = lane & 15, q = lane >> 4;
+  const int piece = lane % PIECES, n = n_wave + piece * 8;
+  float bias[8], scale[8];
+  linear_columns<OUT, S8>(p, n, bias, scale);
+  AccV *own = reinterpret_cast<AccV *>(lds);
+#pragma unroll
+  for (int chunk = 0; chunk < RBW / CHUNK; ++chunk) {
+#pragma unroll
+    for (int b = 0; b < CHUNK; ++b)
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) {
+        const int unit = XT ? nb * 4 + q : (nb >> 1) * 8 + q * 2 + (nb & 1);
+        own[(b * 16 + i) * UNITS + (unit ^ (i & (UNITS - 1)))] = acc[chunk * CHUNK + b][nb];
+      }
+    asm volatile("" ::: "memory");      // (other lanes' units: written above, in order)
+    const int64_t m_chunk = m_wave + chunk * CHUNK * 16;
+#pragma unroll 2
+    for (int r = lane / PIECES; r < CHUNK * 16; r += ROWS) {
+      const AccV *at = own + r * UNITS;
+      const AccV a = at[(2 * piece) ^ (r & (UNITS - 1))], b = at[(2 * piece + 1) ^ (r & (UNITS - 1))];
+      const int64_t m = m_chunk + r;
+      if (m >= p.m || n >= p.n) continue;
+      if (p.partial != nullptr) {      // 32-bit sums of this slice (8-bit operands: whole numbers)
+        const int64_t n8 = (p.n + 7) & ~7;
+        v4i *to = reinterpret_cast<v4i *>(p.partial) + (((int64_t)blockIdx.y * p.m + m) * n8 + n) / 4;
+        to[0] = __builtin_bit_cast(v4i, a);
+        to[1] = __builtin_bit_cast(v4i, b);
+        continue;
+      }
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (float)a[e], v[4 + e] = (float)b[e];
+      linear_finish8<OUT, S8, NT>(p, m, n, v, bias, scale);
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+
+// ---- operands
+
+// One operand of a tile, as DenseOperand lays it out, behind a descriptor that moves along k, BK of it a step.  What a
+// chunk of 16 bytes holds behind the end of k or of the rows has to be there and, where both operands reach it, zero:
+// the host sees to that (linear_repack_kernel).
+template <int ROWS, int KS, int WAVES, bool TR, int SLAB_BLOCKS, bool WIDE_ORDER>
+struct LinearOperand : DenseOperand<ROWS, KS, WAVES, TR, SLAB_BLOCKS, WIDE_ORDER> {
+  using Base = DenseOperand<ROWS, KS, WAVES, TR, SLAB_BLOCKS, WIDE_ORDER>;
+  using Base::voff;
+  using Base::kpos;
+  uint64_t at;       // where the next step begins
+  int64_t left;      // k from there on
+  uint64_t step;     // bytes
+
+  // rows first .. first + ROWS of `count`, from step `s0` on
+  __device__ __forceinline__ void begin(int wave, int lane, const void *ptr, int64_t first, int64_t count, int64_t ld, int64_t k, int64_t s0) {
+    const int rows_here = (int)(count - first < ROWS ? count - first : ROWS);
+#pragma unroll
+    for (int t = 0; t < Base::IP; ++t) {
+      const int slot = (wave * Base::IP + t) * 64 + lane;
+      if constexpr (TR) {
+        const int e = slot / Base::CPR, c = (slot % Base::CPR) ^ Base::swap_tr(e);
+        kpos[t] = e;
+        voff[t] = c * 8 < rows_here ? (uint32_t)(e * ld) + (uint32_t)c * 16u : Base::kOob;
+      } else {
+        const int rho = slot / Base::LPR, c = (slot % Base::LPR) ^ Base::swap_kc(rho);
+        const int i = rho & 15, nb = (rho >> 4) % SLAB_BLOCKS, slab = rho / (16 * SLAB_BLOCKS);
+        const int row = WIDE_ORDER ? slab * (16 * SLAB_BLOCKS) + (nb >> 1) * 32 + (i >> 2) * 8 + (nb & 1) * 4 + (i & 3) : rho;
+        kpos[t] = c * 8;
+        voff[t] = row < rows_here ? (uint32_t)(row * ld) + (uint32_t)c * 16u : Base::kOob;
+      }
+    }
+    step = (uint64_t)(TR ? (int64_t)Base::BK * ld : (int64_t)Base::BK * 2);
+    at = (uint64_t)ptr + (uint64_t)(TR ? first * 2 : first * ld) + (uint64_t)s0 * step;
+    left = k - s0 * Base::BK;
+  }
+  // the next step, into the stage at `lds`; one that is not live is zeros, without traffic
+  __device__ __forceinline__ void issue_next(uint32_t lds, int wave, bool live) {
+    const v4i rsrc = {(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), live ? 0x7fffffff : 0, 0x00020000};
+    if (left >= Base::BK) {
+#pragma unroll
+      for (int t = 0; t < Base::IP; ++t) dma_b128(rsrc, lds + (wave * Base::IP + t) * 1024, voff[t], 0u);
+    } else {
+      const int here = left < 0 ? 0 : (int)left;
+#pragma unroll
+      for (int t = 0; t < Base::IP; ++t) dma_b128(rsrc, lds + (wave * Base::IP + t) * 1024, kpos[t] < here ? voff[t] : Base::kOob, 0u);
+    }
+    skip(1);
+  }
+  __device__ __forceinline__ void skip(int steps) {
+    at += step * (uint64_t)steps;
+    left -= (int64_t)steps * Base::BK;
+  }
+};
+
+// The steps of slice blockIdx.y: whole steps, the last slice takes what is left
+struct LinearSlice {
+  int first, steps;
+};
+__device__ __forceinline__ LinearSlice linear_slice(const LinearParams &p, int step) {
+  const int all = (int)((p.k + step - 1) / step), per = (all + p.slices - 1) / p.slices, first = (int)blockIdx.y * per;
+  const int end = first + per < all ? first + per : all;
+  return {first, end > first ? end - first : 0};
+}
+
+// ---- tiles of WM x WN wave tiles times WK groups of waves that share a step's slices (densegemm_lds_kernel's loop)
+template <class T, class OUT, int WM, int WN, int WK, int RBW, int NBW, int KS, int NS, bool XT, bool YT>
+__global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const LinearParams p, int tiles_m, int tiles_n) {
+  using E = Elem<T>;
+  using AccV = typename E::AccV;
+  constexpr bool S8OP = E::kBytes == 1;
+  static_assert(!S8OP || (!XT && !YT), "8-bit operands are contiguous along k");
+  constexpr int TM = WM * RBW * 16, TN = WN * NBW * 16;
+  using OpY = LinearOperand<TM, KS, WM * WN * WK, YT, RBW, false>;
+  using OpX = LinearOperand<TN, KS, WM * WN * WK, XT, NBW, !XT>;
+  constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
+  constexpr int L = NS - 1;
+  constexpr int WAIT_STEP = (L - 1) * (OpY::IP + OpX::IP);
+  static_assert(WAIT_STEP < 64, "too many loads in flight for the counter");
+  __shared__ __attribute__((aligned(16))) char ring[NS * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wk = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+  constexpr int KW = KS / WK;
+  int tile_m, tile_n;
+  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int64_t m0 = (int64_t)tile_m * TM;
+  const int n0 = tile_n * TN;
+  OpY y;
+  OpX x;
+  const LinearSlice slice = linear_slice(p, OpY::BK);
+  y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
+  x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
+  int y_rd[YT ? RBW : KW], x_rd[XT ? NBW : KW];
+  y.offsets(lane, wm, y_rd, wk * KW);
+  x.offsets(lane, wn, x_rd, wk * KW);
+  AccV acc[RBW][NBW];
+#pragma unroll
+  for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = AccV{0, 0, 0, 0};
+  const uint32_t ring_at = lds_addr(ring);
+  auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+    const bool live = s < slice.steps;
+    const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
+    y.issue_next(st, wave, live);
+    x.issue_next(st + OpY::VECS * 16, wave, live);
+  };
+  for (int s = 0; s < L; ++s) issue(s, s);
+  int cs = 0, ls = L;
+  for (int s = 0; s < slice.steps; ++s) {
+    wait_vmcnt<WAIT_STEP>();
+    lds_barrier();
+    const char *st = ring + cs * STAGE;
+    v4i yf[RBW][KW], xf[NBW][KW];
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb)
+#pragma unroll
+      for (int k = 0; k < KW; ++k) xf[nb][k] = OpX::fragment(st + OpY::VECS * 16 + (XT ? wk * KW * 32 * TN * 2 : 0), x_rd, k, nb);
+#pragma unroll
+    for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+      for (int k = 0; k < KW; ++k) yf[rb][k] = OpY::fragment(st + (YT ? wk * KW * 32 * TM * 2 : 0), y_rd, k, rb);
+    issue(s + L, ls);
+    cs = cs + 1 == NS ? 0 : cs + 1;
+    ls = ls + 1 == NS ? 0 : ls + 1;
+#pragma unroll
+    for (int k = 0; k < KW; ++k)
+#pragma unroll
+      for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+        for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = E::mfma(xf[nb][k], yf[rb][k], acc[rb][nb]);
+  }
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): this wave has read its last stage,
+  lds_barrier();                          // and so has every other
+  constexpr int SHARE = NS * STAGE / (WM * WN * WK);
+  if constexpr (WK == 1) {
+    linear_epilogue<OUT, S8OP, RBW, NBW, XT, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE);
+  } else {
+    // each group finishes its share of the row blocks: it adds up all groups' sums of them, in group order
+    constexpr int RO = RBW / WK;
+    static_assert(RBW % WK == 0 && NS * STAGE >= WM * WN * WK * RBW * NBW * 1024, "the ring holds every group's sums");
+    AccV own[RO][NBW];
+    AccV *park = reinterpret_cast<AccV *>(ring);   // [group][wave of the group][rb][nb][lane]
+    const int wg = wave % (WM * WN);
+#pragma unroll
+    for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) park[(((wk * (WM * WN) + wg) * RBW + rb) * NBW + nb) * 64 + lane] = acc[rb][nb];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RO; ++r)
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) {
+        AccV t = park[((wg * RBW + wk * RO + r) * NBW + nb) * 64 + lane];
+#pragma unroll
+        for (int g = 1; g < WK; ++g) t += park[(((g * (WM * WN) + wg) * RBW + wk * RO + r) * NBW + nb) * 64 + lane];
+        own[r][nb] = t;
+      }
+    __syncthreads();
+    linear_epilogue<OUT, S8OP, RO, NBW, XT, false, SHARE>(p, own, m0 + wm * (RBW * 16) + wk * RO * 16, n0 + wn * (NBW * 16), lane,
+                                                          ring + wave * SHARE);
+  }
+}
+
+// ---- the large tile, its fragments double-buffered in registers (densegemm_pipe_kernel's loop): while the products of a
+// step run on one set, those of the next are read into the other; loads run NS steps ahead
+template <class T, class OUT, int WM, int WN, int RBW, int NBW, int NS, bool XT, bool YT>
+__global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearParams p, int tiles_m, int tiles_n) {
+  using E = Elem<T>;
+  using AccV = typename E::AccV;
+  constexpr bool S8OP = E::kBytes == 1;
+  static_assert(!S8OP || (!XT && !YT), "8-bit operands are contiguous along k");
+  constexpr int TM = WM * RBW * 16, TN = WN * NBW * 16;
+  using OpY = LinearOperand<TM, 1, WM * WN, YT, RBW, false>;
+  using OpX = LinearOperand<TN, 1, WM * WN, XT, NBW, !XT>;
+  constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
+  constexpr int PER = OpY::IP + OpX::IP;
+  __shared__ __attribute__((aligned(16))) char ring[NS * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int tile_m, tile_n;
+  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int64_t m0 = (int64_t)tile_m * TM;
+  const int n0 = tile_n * TN;
+  OpY y;
+  OpX x;
+  const LinearSlice slice = linear_slice(p, OpY::BK);
+  y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
+  x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
+  int y_rd[YT ? RBW : 1], x_rd[XT ? NBW : 1];
+  y.offsets(lane, wm, y_rd);
+  x.offsets(lane, wn, x_rd);
+  AccV acc[RBW][NBW];
+#pragma unroll
+  for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = AccV{0, 0, 0, 0};
+  const uint32_t ring_at = lds_addr(ring);
+  auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+    const bool live = s < slice.steps;
+    const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
+    y.issue_next(st, wave, live);
+    x.issue_next(st + OpY::VECS * 16, wave, live);
+  };
+  v4i ya[RBW], xa[NBW], yb[RBW], xb[NBW];   // the fragments of two steps
+  auto read = [&](int stage, v4i (&yf)[RBW], v4i (&xf)[NBW]) __attribute__((always_inline)) {
+    const char *st = ring + stage * STAGE;
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) xf[nb] = OpX::fragment(st + OpY::VECS * 16, x_rd, 0, nb);
+#pragma unroll
+    for (int rb = 0; rb < RBW; ++rb) yf[rb] = OpY::fragment(st, y_rd, 0, rb);
+  };
+  for (int s = 0; s < NS; ++s) issue(s, s);
+  wait_vmcnt<(NS - 1) * PER>();
+  lds_barrier();
+  read(0, ya, xa);
+  int cs = 0;
+  auto phase = [&](int s, v4i (&yc)[RBW], v4i (&xc)[NBW], v4i (&yn)[RBW], v4i (&xn)[NBW]) __attribute__((always_inline)) {
+    wait_vmcnt<(NS - 2) * PER>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): the fragments of step s are in registers
+    lds_barrier();
+    issue(s + NS, cs);
+    cs = cs + 1 == NS ? 0 : cs + 1;
+    read(cs, yn, xn);
+#pragma unroll
+    for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = E::mfma(xc[nb], yc[rb], acc[rb][nb]);
+    // (reads and products interleaved: the scheduler would put all reads first)
+    constexpr int READS = RBW * (YT ? 2 : 1) + NBW * (XT ? 2 : 1);
+    constexpr int MF = RBW * NBW;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, MF / READS > 0 ? MF / READS : 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
+  };
+  int s = 0;
+  for (; s + 1 < slice.steps; s += 2) {
+    phase(s, ya, xa, yb, xb);
+    phase(s + 1, yb, xb, ya, xa);
+  }
+  if (s < slice.steps) phase(s, ya, xa, yb, xb);
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  lds_barrier();
+  constexpr int SHARE = NS * STAGE / (WM * WN);
+  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE);
+}
+
+// ---- few rows: MB blocks of 16 of them, 16 columns per workgroup, the steps dealt out to its W waves.  What counts is the
+// weight, read once from memory: every wave streams its share of 16 weight rows through a ring of its own, no barrier,
+// no wait for others; the waves' sums are added up in LDS in wave order.
+template <class T, class OUT, int W, int MB, int KS, int NS>
+__global__ __launch_bounds__(W * 64) void linear_few_kernel(const LinearParams p) {
+  using E = Elem<T>;
+  using AccV = typename E::AccV;
+  constexpr bool S8OP = E::kBytes == 1;
+  using OpY = LinearOperand<MB * 16, KS, 1, false, MB, false>;
+  using OpX = LinearOperand<16, KS, 1, false, 1, false>;
+  constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
+  constexpr int L = NS - 1, PER = OpY::IP + OpX::IP;
+  static_assert(L * PER < 64 && NS * STAGE >= MB * 1024, "the ring holds a wave's sums");
+  __shared__ __attribute__((aligned(16))) char ring[W][NS * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = (int)blockIdx.x * 16;
+  OpY y;
+  OpX x;
+  y.begin(0, lane, p.Y, 0, p.m, p.ldy, p.k, wave);
+  x.begin(0, lane, p.X, n0, p.n, p.ldx, p.k, wave);
+  int y_rd[KS], x_rd[KS];
+  y.offsets(lane, 0, y_rd);
+  x.offsets(lane, 0, x_rd);
+  const int steps = (int)((p.k + OpY::BK - 1) / OpY::BK), mine = steps > wave ? (steps - wave + W - 1) / W : 0;
+  AccV acc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) acc[b] = AccV{0, 0, 0, 0};
+  const uint32_t ring_at = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(&ring[wave][0]));
+  auto issue = [&](int j, int stage) __attribute__((always_inline)) {
+    const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
+    y.issue_next(st, 0, j < mine);
+    x.issue_next(st + OpY::VECS * 16, 0, j < mine);
+    y.skip(W - 1);      // (the other waves' steps)
+    x.skip(W - 1);
+  };
+  for (int j = 0; j < L; ++j) issue(j, j);
+  int cs = 0, ls = L;
+  for (int j = 0; j < mine; ++j) {
+    wait_vmcnt<(L - 1) * PER>();
+    asm volatile("" ::: "memory");
+    const char *st = &ring[wave][cs * STAGE];
+    v4i yf[MB][KS], xf[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) xf[k] = OpX::fragment(st + OpY::VECS * 16, x_rd, k, 0);
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) yf[b][k] = OpY::fragment(st, y_rd, k, b);
+    issue(j + L, ls);
+    cs = cs + 1 == NS ? 0 : cs + 1;
+    ls = ls + 1 == NS ? 0 : ls + 1;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int b = 0; b < MB; ++b) acc[b] = E::mfma(xf[k], yf[b][k], acc[b]);
+  }
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("" ::: "memory");
+  // every wave parks its sums in its own ring: [row][column], 16 of each per block
+  const int i = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < MB; ++b) reinterpret_cast<AccV *>(&ring[wave][0])[(b * 16 + i) * 4 + q] = acc[b];
+  __syncthreads();
+  for (int t = tid; t < MB * 32; t += W * 64) {
+    const int m = t >> 1, half = t & 1;
+    if (m >= p.m || n0 + half * 8 >= p.n) continue;
+    AccV a = reinterpret_cast<const AccV *>(&ring[0][0])[m * 4 + half * 2], b = reinterpret_cast<const AccV *>(&ring[0][0])[m * 4 + half * 2 + 1];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      a += reinterpret_cast<const AccV *>(&ring[w][0])[m * 4 + half * 2];
+      b += reinterpret_cast<const AccV *>(&ring[w][0])[m * 4 + half * 2 + 1];
+    }
+    float v[8], bias[8], scale[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)a[e], v[4 + e] = (float)b[e];
+    linear_columns<OUT, S8OP>(p, n0 + half * 8, bias, scale);
+    linear_finish8<OUT, S8OP, false>(p, m, n0 + half * 8, v, bias, scale);
+  }
+}
+
+// The slices' sums added up, and the epilogue: eight columns of a row by LANES threads, which take every LANES-th slice in
+// order and are then added up in order themselves (few outputs and many slices: a chain of loads is LANES times as short)
+template <class OUT, bool S8, int LANES>
+__global__ __launch_bounds__(256) void linear_join_kernel(const LinearParams p) {
+  typedef std::conditional_t<S8, v4i, v4f> V;
+  constexpr int ITEMS = 256 / LANES;
+  __shared__ V lds[LANES > 1 ? 2 * 256 : 1];
+  const int pieces = (p.n + 7) >> 3, item = threadIdx.x % ITEMS, part = threadIdx.x / ITEMS;
+  const int64_t i = (int64_t)blockIdx.x * ITEMS + item, all = p.m * pieces;
+  const V *at = reinterpret_cast<const V *>(p.partial) + i * 2;
+  V a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+  if (i < all) {
+#pragma unroll 4
+    for (int s = part; s < p.slices; s += LANES) {
+      a += at[s * all * 2];
+      b += at[s * all * 2 + 1];
+    }
+  }
+  if constexpr (LANES > 1) {
+    lds[threadIdx.x * 2] = a;
+    lds[threadIdx.x * 2 + 1] = b;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int l = 1; l < LANES; ++l) {
+      a += lds[(l * ITEMS + item) * 2];
+      b += lds[(l * ITEMS + item) * 2 + 1];
+    }
+  }
+  if (i >= all) return;
+  const int64_t m = i / pieces;
+  const int n = (int)(i - m * pieces) * 8;
+  float v[8], bias[8], scale[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)a[e], v[4 + e] = (float)b[e];
+  linear_columns<OUT, S8>(p, n, bias, scale);
+  linear_finish8<OUT, S8, false>(p, m, n, v, bias, scale);
+}
+
+// An operand whose rows do not lie on 16-byte borders, or end between them: a copy whose rows do, zeros behind their
+// ends.  thread = 16 bytes of a row of `to`, ES bytes an element
+template <int ES>
+__global__ __launch_bounds__(256) void linear_repack_kernel(v4i *to, const void *from, int64_t rows, int64_t cols, int64_t ld, int64_t pieces, int64_t to_ld) {
+  using U = std::conditional_t<ES == 1, uint8_t, uint16_t>;
+  constexpr int PER = 16 / ES;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * pieces; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / pieces, c = (t - r * pieces) * PER;
+    const U *src = reinterpret_cast<const U *>(from) + r * ld + c;
+    v4i v;
+    U *u = reinterpret_cast<U *>(&v);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) u[e] = c + e < cols ? src[e] : (U)0;
+    to[r * (to_ld / 16) + c / PER] = v;
+  }
+}
+
+}  // namespace cummhip

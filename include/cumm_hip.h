@@ -523,6 +523,91 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
                                 int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 
+/* ---- row-wise layers around the products.  The reference has none of them: its matmul2 adds a bias or a matrix to the
+ * sum and applies the activation to both, and its int8 inference epilogue takes scales that somebody has made.
+ * Types f16 and bf16 (dtype), and what each entry names beside them; every sum, norm and scale is 32 bits, every result is
+ * rounded once.  Rows may be any number of elements apart (ld*), at any alignment of an element; operands whose rows do
+ * not lie on 16-byte borders, or are no multiple of 16 bytes long, are copied into the workspace first.  Rows of m up to
+ * 2^31 - 1, of less than 8 MiB each; nothing else is limited.  Nothing is allocated, no stream waited for; calls that may
+ * overlap in time need a workspace each (*_workspace bytes, 256-byte aligned; -1 for arguments that are not taken).
+ *
+ * cumm_hip_linear:  out[r][c] = act(sum_k x[r][k] weight[c][k] + bias[c]) + residual[r][c]
+ *   dtype CUMM_HIP_S8: x and weight are whole numbers of 8 bits, the sum (exact below 2^31: k up to 131071) times x_scale[r]
+ *   weight_scale[c]; bias is f32 then, residual and out are of out_dtype.  (Otherwise bias, residual and out are of dtype.)
+ *   pre_act, unless NULL, gets what the activation gets (rounded): the backward pass wants it.
+ *   out may be residual itself, with its pitch; apart from that no output overlaps an operand.
+ *   m == 0 is no work; NaN passes through every activation.
+ * cumm_hip_linear_backward: the gradients for grad_out [m, n], each NULL where it is not wanted:
+ *     dz = grad_out act'(pre_act);  grad_x = dz weight [m, k];  grad_weight = dz^T x [n, k];  grad_bias = sum of dz's rows
+ *   (the residual's is grad_out).  dz is rounded to dtype for the two products, not for the sum.  pre_act NULL: only with
+ *   CUMM_HIP_ACT_NONE; for CUMM_HIP_ACT_RELU without a residual, out serves as well.  m == 0 gives zeros. */
+#define CUMM_HIP_ACT_SILU 4
+#define CUMM_HIP_ACT_GELU 5        /* x Phi(x), by erf */
+#define CUMM_HIP_ACT_GELU_TANH 6
+typedef struct CummHipLinearArgs {
+  int32_t dtype, out_dtype;
+  int64_t m;
+  int32_t n, k;
+  const void *x, *weight, *bias, *residual;      /* [m, k], [n, k], [n] or NULL, [m, n] or NULL */
+  void *out, *pre_act;                           /* [m, n], [m, n] or NULL */
+  int64_t ld_x, ld_weight, ld_residual, ld_out, ld_pre_act;   /* elements between rows */
+  const float *x_scale, *weight_scale;           /* [m], [n]: CUMM_HIP_S8 */
+  int32_t act_type;
+  float act_alpha;                               /* slope of CUMM_HIP_ACT_LEAKY_RELU */
+  void *workspace;
+  size_t workspace_bytes;
+} CummHipLinearArgs;
+int64_t cumm_hip_linear_workspace(const CummHipLinearArgs *args);
+int cumm_hip_linear(const CummHipLinearArgs *args, void *stream);
+typedef struct CummHipLinearGradArgs {
+  int32_t dtype;
+  int64_t m;
+  int32_t n, k;
+  const void *grad_out, *pre_act, *x, *weight;
+  int64_t ld_grad_out, ld_pre_act, ld_x, ld_weight;
+  void *grad_x, *grad_weight, *grad_bias;        /* dense */
+  int32_t act_type;
+  float act_alpha;
+  void *workspace;
+  size_t workspace_bytes;
+} CummHipLinearGradArgs;
+int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *args);
+int cumm_hip_linear_backward(const CummHipLinearGradArgs *args, void *stream);
+
+/* cumm_hip_rms_norm:  total = x + residual (rounded to dtype; x itself where residual is NULL), and of that
+ *     inv = 1 / sqrt(mean over the row of total^2 + eps),  out = total * inv * weight
+ *   or, where codes is given instead of out, out in 8 bits: v = total * weight, top = the row's largest |v|, a code is the
+ *   whole number next to 127 v / top (ties to even), scale = inv * top / 127 of the row: code * scale stands for out.
+ *   weight NULL (with codes, without residual; dtype may then be CUMM_HIP_F32 too): rows in 8 bits without a norm, inv = 1.
+ *   A row of zeros has codes 0 and scale 0; one with an infinity or a NaN has codes 0 and the scale that comes of it (an
+ *   infinity or NaN), so that no wrong finite value results.  inv_rms [m], unless NULL, gets inv.  eps > 0.
+ * cumm_hip_rms_norm_backward: for the gradients of out and of total (either NULL: zeros),
+ *     grad_x = inv (grad_out weight - u mean of grad_out weight u) + grad_total, u = total inv  (it is the residual's too)
+ *     grad_weight = sum over rows of grad_out u       each NULL where it is not wanted */
+typedef struct CummHipRmsNormArgs {
+  int32_t dtype, k;
+  int64_t m;
+  const void *x, *residual, *weight;             /* [m, k], [m, k] or NULL, [k] or NULL */
+  int64_t ld_x, ld_residual;
+  void *out, *total;                             /* [m, k] dense; total NULL without residual */
+  int8_t *codes;                                 /* [m, k] dense, instead of out */
+  float *scale, *inv_rms;                        /* [m] */
+  float eps;
+} CummHipRmsNormArgs;
+int cumm_hip_rms_norm(const CummHipRmsNormArgs *args, void *stream);
+typedef struct CummHipRmsNormGradArgs {
+  int32_t dtype, k;
+  int64_t m;
+  const void *total, *weight, *grad_out, *grad_total;
+  int64_t ld_total, ld_grad_out, ld_grad_total;
+  const float *inv_rms;
+  void *grad_x, *grad_weight;                    /* dense */
+  void *workspace;
+  size_t workspace_bytes;
+} CummHipRmsNormGradArgs;
+int64_t cumm_hip_rms_norm_backward_workspace(const CummHipRmsNormGradArgs *args);
+int cumm_hip_rms_norm_backward(const CummHipRmsNormGradArgs *args, void *stream);
+
 /* Plain device-to-device copy kernel of `bytes` bytes (16-byte aligned); used to
  * calibrate the HBM traffic counters against a transfer of known size. */
 int cumm_hip_copy_kernel(void *dst, const void *src, size_t bytes, void *stream);
