@@ -103,7 +103,7 @@ def _torch_native_stamp():
     """What the native half was built from: its source, the interface it shares with the library and torch."""
     import torch
     h = hashlib.sha256()
-    for f in (TORCH_SRC, os.path.join(HERE, "..", "include", "cumm_hip.h")):
+    for f in (TORCH_SRC, os.path.join(CSRC, "torch_layers.h"), os.path.join(HERE, "..", "include", "cumm_hip.h")):
         with open(f, "rb") as stream:
             h.update(stream.read())
     h.update(("%s %s" % (torch.__version__, sys.implementation.cache_tag)).encode())

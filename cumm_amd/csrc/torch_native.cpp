@@ -14,7 +14,9 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/util/Exception.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/dynamo/compiled_autograd.h>
@@ -53,6 +55,13 @@ struct Api {
   CUMM_API(conv_pairs_fill);
   CUMM_API(order_pairs_coarse);
   CUMM_API(order_pairs_coarse_workspace);
+  CUMM_API(linear);
+  CUMM_API(linear_workspace);
+  CUMM_API(linear_backward);
+  CUMM_API(linear_backward_workspace);
+  CUMM_API(rms_norm);
+  CUMM_API(rms_norm_backward);
+  CUMM_API(rms_norm_backward_workspace);
 #undef CUMM_API
 } api;
 
@@ -74,6 +83,13 @@ void bind(const py::dict &addresses) {
   CUMM_API(conv_pairs_fill);
   CUMM_API(order_pairs_coarse);
   CUMM_API(order_pairs_coarse_workspace);
+  CUMM_API(linear);
+  CUMM_API(linear_workspace);
+  CUMM_API(linear_backward);
+  CUMM_API(linear_backward_workspace);
+  CUMM_API(rms_norm);
+  CUMM_API(rms_norm_backward);
+  CUMM_API(rms_norm_backward_workspace);
 #undef CUMM_API
 }
 
@@ -560,6 +576,8 @@ py::object forward(const Tensor &features, const Tensor &weight, const std::opti
   return result.defined() ? py::cast(result) : py::none();
 }
 
+#include "torch_layers.h"
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -592,4 +610,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("remember", &remember);
   m.def("build", &build);
   m.def("forward", &forward);
+  m.def("layer_linear", &layer_linear);
+  m.def("layer_linear_s8", &layer_linear_s8);
+  m.def("layer_norm", &layer_norm_);
+  m.def("layer_quantize", &layer_quantize);
 }

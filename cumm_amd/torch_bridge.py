@@ -170,7 +170,8 @@ _KINDS = {}
 _NATIVE_SYMBOLS = ("sparse_conv_more", "last_error", "relu_backward", "gate_sums", "column_sum_workspace",
                    "query_conv_workspace", "query_wgrad_ordered_workspace", "wgrad_pairs_sums", "wgrad_pairs_workspace", "subm_pairs",
                    "subm_pairs_workspace", "conv_pairs_workspace", "conv_pairs_sites", "conv_pairs_fill", "order_pairs_coarse",
-                   "order_pairs_coarse_workspace")
+                   "order_pairs_coarse_workspace", "linear", "linear_workspace", "linear_backward", "linear_backward_workspace", "rms_norm",
+                   "rms_norm_backward", "rms_norm_backward_workspace")
 _native_module = None
 
 

@@ -14,7 +14,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _capi
+from . import _capi, torch_bridge
 from . import tensorview as tv
 
 ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "leaky_relu": 3, "silu": 4, "gelu": 5, "gelu_tanh": 6}
@@ -25,6 +25,14 @@ _HALVES = (torch.float16, torch.bfloat16)
 def _check(ok: bool, text: str) -> None:
     if not ok:
         raise ValueError(text)
+
+
+def _native():
+    """The native half (csrc/torch_layers.h), which makes the calls that it can: everything else, and all of them where there
+    is none, is made here."""
+    if torch._C._are_functorch_transforms_active() or torch.compiler.is_compiling():
+        return None
+    return torch_bridge._native()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -169,6 +177,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None, slope: float = 0.01) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual`` for x [..., K], weight [N, K] (f16 / bf16); one rounding.  Differentiable in
     all four tensors (once).  ``slope`` is that of "leaky_relu"."""
+    native = _native()
+    if native is not None and activation in ACTIVATIONS:
+        out = native.layer_linear(x, weight, bias, residual, ACTIVATIONS[activation], slope)
+        if out is not None:
+            return out
     _check(x.dtype in _HALVES, "linear: x must be float16 or bfloat16 (linear_s8 takes 8-bit rows)")
     shape = x.shape[:-1] + weight.shape[:1]
     x, weight, bias, residual, act = _linear_args("linear", x, weight, bias, residual, activation, x.dtype, x.dtype)
@@ -185,6 +198,11 @@ def linear_s8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     """The same for 8-bit rows: x [..., K] and weight [N, K] int8 with the scales of their rows (float32: x_scale [...],
     weight_scale [N], as ``quantize_rows`` and ``rms_norm_s8`` give them), bias float32, residual and result ``dtype``.
     Inference only: it has no gradient.  K up to 131071 (the sums of products are whole numbers of 32 bits)."""
+    native = _native()
+    if native is not None and activation in ACTIVATIONS:
+        out = native.layer_linear_s8(x, x_scale, weight, weight_scale, bias, residual, ACTIVATIONS[activation], slope, dtype)
+        if out is not None:
+            return out
     _check(x.dtype == torch.int8, "linear_s8: x must be int8")
     _check(dtype in _HALVES, "linear_s8: dtype must be float16 or bfloat16")
     shape = x.shape[:-1] + weight.shape[:1]
@@ -278,6 +296,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
              residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``h / sqrt(mean(h^2) + eps) * weight`` over the last dimension of ``h = x``; with a residual ``h = x + residual``, rounded
     to the tensors' type, and (result, h) comes back.  Differentiable in all tensors (once)."""
+    native = _native()
+    if native is not None:
+        got = native.layer_norm(x, weight, residual, eps, False)
+        if got is not None:
+            return got
     shape = x.shape
     x, weight, residual = _norm_args("rms_norm", x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
@@ -294,6 +317,11 @@ def rms_norm_s8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, res
     """The norm with its result in 8 bits: (codes int8, scale float32 of every row), and h with a residual; code * scale
     stands for the result.  A row's largest magnitude is 127; a row of zeros has scale 0, one with an infinity or a NaN a scale
     that is not finite.  Inference only."""
+    native = _native()
+    if native is not None:
+        got = native.layer_norm(x, weight, residual, eps, True)
+        if got is not None:
+            return got
     _no_gradient("rms_norm_s8", x, weight, residual)
     shape = x.shape
     x, weight, residual = _norm_args("rms_norm_s8", x, weight, residual, eps)
@@ -305,6 +333,11 @@ def rms_norm_s8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, res
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [..., K] (f16, bf16 or f32) in 8 bits: (codes int8, scale float32 [...]), as ``rms_norm_s8`` gives them.  For weights
     [N, K] of ``linear_s8`` and activations between two products."""
+    native = _native()
+    if native is not None:
+        got = native.layer_quantize(x)
+        if got is not None:
+            return got
     _no_gradient("quantize_rows", x)
     _check(x.dim() >= 1 and x.shape[-1] > 0, "quantize_rows: x must be [..., K]")
     _check(x.dtype in _HALVES or x.dtype == torch.float32, "quantize_rows: x must be float16, bfloat16 or float32")

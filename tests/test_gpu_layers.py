@@ -21,8 +21,18 @@ ACTS = ["none", "relu", "sigmoid", "leaky_relu", "silu", "gelu", "gelu_tanh"]
 
 @pytest.fixture(scope="module")
 def L():
-    from cumm_amd import torch_layers
+    from cumm_amd import torch_bridge, torch_layers
+    assert torch_bridge._native() is not None
     return torch_layers
+
+
+@pytest.fixture(params=["native", "python"])
+def either(request, L, monkeypatch):
+    """The layers, and as a machine without a host compiler has them."""
+    if request.param == "python":
+        from cumm_amd import torch_bridge
+        monkeypatch.setattr(torch_bridge, "_native_module", False)
+    return L
 
 
 def gen(seed):
@@ -99,7 +109,8 @@ def test_linear_large_tile(L):
     linear_case(L, torch.float16, 4100, 520, 4001, "relu", True, False)
 
 
-def test_linear_shapes_and_empty(L):
+def test_linear_shapes_and_empty(either):
+    L = either
     g = gen(1)
     x, w, b = normal(g, 2, 3, 5, 40), normal(g, 24, 40), normal(g, 24)
     got = L.linear(x, w, b)
@@ -186,7 +197,8 @@ def test_linear_gradient_against_differences(L, act):
 
 
 @pytest.mark.parametrize("wanted", ["x", "w", "b", "r", "xw", "wb", "xb"])
-def test_linear_some_gradients(L, wanted):
+def test_linear_some_gradients(either, wanted):
+    L = either
     g = gen(5)
     t = dict(x=normal(g, 90, 40), w=normal(g, 56, 40), b=normal(g, 56), r=normal(g, 90, 56))
     dy = normal(g, 90, 56)
@@ -200,8 +212,9 @@ def test_linear_some_gradients(L, wanted):
         assert torch.equal(some[name], all_of_them[name]), name
 
 
-def test_linear_gradient_of_strided_and_broadcast_results(L):
+def test_linear_gradient_of_strided_and_broadcast_results(either):
     """A gradient that is a number spread out, or a transposed view; leading dimensions; no rows at all."""
+    L = either
     g = gen(6)
     x, w, b = (t.requires_grad_() for t in (normal(g, 4, 9, 40), normal(g, 24, 40), normal(g, 24)))
     dy = normal(g, 9, 24, 4).permute(2, 0, 1)
@@ -389,8 +402,9 @@ def test_norm_gradient_against_differences(L):
             assert abs(float(got[i, j]) - float(want)) <= abs(float(want)) * EPS[torch.float16] + 1e-5
 
 
-def test_norm_gradients_of_one_result_only(L):
+def test_norm_gradients_of_one_result_only(either):
     """A gradient of the sum alone, or of the norm alone, or with parts that want none."""
+    L = either
     g = gen(4)
     x, r, w = (normal(g, 12, 72).requires_grad_(), normal(g, 12, 72).requires_grad_(), normal(g, 72).requires_grad_())
     dy = normal(g, 12, 72)
@@ -408,7 +422,8 @@ def test_norm_gradients_of_one_result_only(L):
     assert (torch.autograd.grad(empty, w, dy[:0])[0] == 0).all()
 
 
-def test_same_bits_from_run_to_run(L):
+def test_same_bits_from_run_to_run(either):
+    L = either
     g = gen(11)
     x, w, b = (t.requires_grad_() for t in (normal(g, 3000, 96), normal(g, 136, 96), normal(g, 136)))
     n = normal(g, 96).requires_grad_()
@@ -464,8 +479,9 @@ def test_block_in_8_bits(L, dtype, m):
     assert float((got.double() - h.double() - full).norm() / full.norm()) < 0.05
 
 
-def test_block_trains(L):
+def test_block_trains(either):
     """Norm, two products and the residual stream, forward and backward, against the formula's gradients in 64 bits."""
+    L = either
     torch.manual_seed(0)
     norm, up, down = L.RMSNorm(96, dtype=torch.bfloat16), L.Linear(96, 200, activation="gelu_tanh", dtype=torch.bfloat16), L.Linear(200, 96, dtype=torch.bfloat16)
     x = torch.randn(3, 50, 96, device="cuda").bfloat16().requires_grad_()
@@ -510,8 +526,9 @@ def test_captured_inference(L, m):
     replays(run, [x, skip], run)
 
 
-def test_captured_training_step(L):
+def test_captured_training_step(either):
     """Forward and backward of the same leaves in one graph; eager passes take leaves of their own."""
+    L = either
     g = gen(2)
     shapes = [(200, 72), (72,), (130, 72), (130,), (200, 130)]
     t = [normal(g, *s).requires_grad_() for s in shapes[:4]] + [normal(g, *shapes[4])]
@@ -598,3 +615,25 @@ def test_more_than_two_gigabytes(L):
     codes, scale = L.quantize_rows(x)
     small = L.quantize_rows(tail)
     assert torch.equal(codes[-300:], small[0]) and torch.equal(scale[-300:], small[1])
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 48), (33, 100, 40), (300, 256, 264)])
+def test_both_halves_give_the_same(L, monkeypatch, m, k, n):
+    from cumm_amd import torch_bridge
+    g = gen(m)
+    x, w, b, r, nw = (t.requires_grad_() for t in (normal(g, m, k), normal(g, n, k, scale=k ** -0.5), normal(g, n), normal(g, m, n), normal(g, k)))
+    dy = normal(g, m, n)
+
+    def all_of_it():
+        h, total = L.rms_norm(x, nw, residual=x.detach())
+        out = L.linear(h, w, b, activation="gelu", residual=r)
+        grads = torch.autograd.grad((out, total), (x, w, b, r, nw), (dy, dy[:, :1].expand(m, k)))
+        with torch.no_grad():
+            codes = L.rms_norm_s8(x, nw, residual=x)
+            q = L.quantize_rows(w)
+            s8 = L.linear_s8(codes[0], codes[1], q[0], q[1], b.float(), activation="silu", residual=r, dtype=torch.float16)
+        return (out, h, total, s8) + grads + codes + q
+    native = all_of_it()
+    monkeypatch.setattr(torch_bridge, "_native_module", False)
+    own = all_of_it()
+    assert len(native) == len(own) and all(torch.equal(a, c) and a.dtype == c.dtype for a, c in zip(native, own))
