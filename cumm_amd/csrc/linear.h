@@ -178,19 +178,20 @@ __device__ __forceinline__ void linear_finish8(const LinearParams &p, int64_t m,
 // of each block, of row i.  They go through the wave's share of LDS (BYTES of it, CHUNK row blocks at a time) and come
 // back as eight consecutive columns a lane: whole lines of 64 or 128 bytes per row and store, and a loop over rows instead
 // of an epilogue written out for every accumulator, which needs more registers than the large tile leaves.  Rows are
-// [row][16 or 8 units of four columns], units permuted by the row: neither side meets a bank twice.
+// [row][16 or 8 units of four columns], units permuted by the row: neither side meets a bank twice.  The residual and the
+// rows' scales are fetched a group of rows ahead (row by row, a round trip to memory each, 8192 x 4096 x 4096 with a
+// residual takes 235 us, 25 more than without; so 218).
 template <class OUT, bool S8, int RBW, int NBW, bool XT, bool NT, int BYTES, class AccV>
 __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const AccV (&acc)[RBW][NBW], int64_t m_wave, int n_wave, int lane, char *lds) {
   constexpr int UNITS = NBW * 4, PIECES = NBW * 2, ROWS = 64 / PIECES;      // ROWS at a time
-  constexpr int FIT = BYTES / (NBW * 1024), CHUNK = FIT < RBW ? FIT : RBW;
-  static_assert((NBW == 2 || NBW == 4) && CHUNK >= 1 && RBW % CHUNK == 0, "row blocks of a chunk");
+  constexpr int FIT = BYTES / (NBW * 1024), CHUNK = FIT >= RBW ? RBW : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
+  constexpr int TIMES = CHUNK * 16 / ROWS, GROUP = TIMES < 4 ? TIMES : 4, GROUPS = TIMES / GROUP, ALL = RBW / CHUNK * GROUPS;
+  static_assert((NBW == 2 || NBW == 4) && FIT >= 1 && RBW % CHUNK == 0 && TIMES % GROUP == 0, "row blocks of a chunk");
   const int i = lane & 15, q = lane >> 4;
-  const int piece = lane % PIECES, n = n_wave + piece * 8;
-  float bias[8], scale[8];
-  linear_columns<OUT, S8>(p, n, bias, scale);
+  const int piece = lane % PIECES, sub = lane / PIECES, n = n_wave + piece * 8, count = p.n - n;
+  const bool in_n = count > 0;
   AccV *own = reinterpret_cast<AccV *>(lds);
-#pragma unroll
-  for (int chunk = 0; chunk < RBW / CHUNK; ++chunk) {
+  const auto park = [&](int chunk) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < CHUNK; ++b)
 #pragma unroll
@@ -199,24 +200,86 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const Acc
         own[(b * 16 + i) * UNITS + (unit ^ (i & (UNITS - 1)))] = acc[chunk * CHUNK + b][nb];
       }
     asm volatile("" ::: "memory");      // (other lanes' units: written above, in order)
-    const int64_t m_chunk = m_wave + chunk * CHUNK * 16;
-#pragma unroll 2
-    for (int r = lane / PIECES; r < CHUNK * 16; r += ROWS) {
-      const AccV *at = own + r * UNITS;
-      const AccV a = at[(2 * piece) ^ (r & (UNITS - 1))], b = at[(2 * piece + 1) ^ (r & (UNITS - 1))];
-      const int64_t m = m_chunk + r;
-      if (m >= p.m || n >= p.n) continue;
-      if (p.partial != nullptr) {      // 32-bit sums of this slice (8-bit operands: whole numbers)
-        const int64_t n8 = (p.n + 7) & ~7;
-        v4i *to = reinterpret_cast<v4i *>(p.partial) + (((int64_t)blockIdx.y * p.m + m) * n8 + n) / 4;
-        to[0] = __builtin_bit_cast(v4i, a);
-        to[1] = __builtin_bit_cast(v4i, b);
-        continue;
-      }
-      float v[8];
+  };
+  const auto take = [&](int r, AccV &a, AccV &b) __attribute__((always_inline)) {
+    const AccV *at = own + r * UNITS;
+    a = at[(2 * piece) ^ (r & (UNITS - 1))];
+    b = at[(2 * piece + 1) ^ (r & (UNITS - 1))];
+  };
+  if (p.partial != nullptr) {      // 32-bit sums of this slice (8-bit operands: whole numbers)
+    const int64_t n8 = (p.n + 7) & ~7;
+    v4i *to = reinterpret_cast<v4i *>(p.partial) + ((int64_t)blockIdx.y * p.m * n8 + n) / 4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)a[e], v[4 + e] = (float)b[e];
-      linear_finish8<OUT, S8, NT>(p, m, n, v, bias, scale);
+    for (int chunk = 0; chunk < RBW / CHUNK; ++chunk) {
+      park(chunk);
+#pragma unroll 4
+      for (int r = sub; r < CHUNK * 16; r += ROWS) {
+        AccV a, b;
+        take(r, a, b);
+        const int64_t m = m_wave + chunk * CHUNK * 16 + r;
+        if (m < p.m && in_n) {
+          to[m * n8 / 4] = __builtin_bit_cast(v4i, a);
+          to[m * n8 / 4 + 1] = __builtin_bit_cast(v4i, b);
+        }
+      }
+      asm volatile("" ::: "memory");
+    }
+    return;
+  }
+  Piece<OUT> add[GROUP];
+  float row[GROUP];
+  const auto fetch = [&](int group) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j) {
+      const int64_t m = m_wave + (group * GROUP + j) * ROWS + sub;
+      const bool in = m < p.m && in_n && group < ALL;
+      add[j].raw = v4i{0, 0, 0, 0};
+      row[j] = 0.0f;
+      if (p.residual != nullptr && in) add[j].load(p.residual, m * p.ldr + n, count);
+      if (S8 && in) row[j] = p.y_scale[m];
+    }
+  };
+  fetch(0);
+  float bias[8], scale[8];
+  linear_columns<OUT, S8>(p, n, bias, scale);
+#pragma unroll
+  for (int chunk = 0; chunk < RBW / CHUNK; ++chunk) {
+    park(chunk);
+#pragma unroll 1
+    for (int g = 0; g < GROUPS; ++g) {
+      float v[GROUP * 8], r[GROUP * 8];
+      const int64_t m0 = m_wave + (chunk * GROUPS + g) * GROUP * ROWS + sub;
+#pragma unroll
+      for (int j = 0; j < GROUP; ++j) {
+        AccV a, b;
+        take((g * GROUP + j) * ROWS + sub, a, b);
+        float t[8];
+        add[j].values(t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float z = (float)(e < 4 ? a[e & 3] : b[e & 3]);
+          v[j * 8 + e] = S8 ? __builtin_fmaf(z * row[j], scale[e], bias[e]) : z + bias[e];
+          r[j * 8 + e] = t[e];
+        }
+      }
+      fetch(chunk * GROUPS + g + 1);
+      const auto store = [&](void *base, int64_t ld) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+          float t[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = v[j * 8 + e];
+          Piece<OUT> out;
+          out.round(t);
+          const int64_t m = m0 + j * ROWS;
+          if (m < p.m && in_n) out.template store<NT>(base, m * ld + n, count);
+        }
+      };
+      if (p.pre != nullptr) store(p.pre, p.ldp);
+      linear_act(v, p.act, p.slope);
+#pragma unroll
+      for (int e = 0; e < GROUP * 8; ++e) v[e] += r[e];
+      store(p.out, p.ldo);
     }
     asm volatile("" ::: "memory");
   }
@@ -387,20 +450,24 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   }
 }
 
-// ---- the large tile, its fragments double-buffered in registers (densegemm_pipe_kernel's loop): while the products of a
-// step run on one set, those of the next are read into the other; loads run NS steps ahead
-template <class T, class OUT, int WM, int WN, int RBW, int NBW, int NS, bool XT, bool YT>
+// ---- the large tile, its fragments double-buffered in registers: while the products of one half of a step (32 k) run on
+// one set, those of the next half are read into the other.  A step is 64 k, so that a row's share of it is a whole line
+// of 128 bytes (with 32 k every line is asked for twice: 8192 x 4096 x 4096 250 us instead of 210), and there are two
+// stages: the loads of step s + 2 begin when the second half of step s is in registers, and have a whole step's products,
+// 2048 clocks of the matrix cores, to arrive.  Without the wait for them the time is the same (204 against 204), without
+// the loads it is 172: what is left of them is their traffic and its power, not their latency.
+template <class T, class OUT, int WM, int WN, int RBW, int NBW, bool XT, bool YT>
 __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearParams p, int tiles_m, int tiles_n) {
   using E = Elem<T>;
   using AccV = typename E::AccV;
   constexpr bool S8OP = E::kBytes == 1;
   static_assert(!S8OP || (!XT && !YT), "8-bit operands are contiguous along k");
   constexpr int TM = WM * RBW * 16, TN = WN * NBW * 16;
-  using OpY = LinearOperand<TM, 1, WM * WN, YT, RBW, false>;
-  using OpX = LinearOperand<TN, 1, WM * WN, XT, NBW, !XT>;
+  using OpY = LinearOperand<TM, 2, WM * WN, YT, RBW, false>;
+  using OpX = LinearOperand<TN, 2, WM * WN, XT, NBW, !XT>;
   constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
   constexpr int PER = OpY::IP + OpX::IP;
-  __shared__ __attribute__((aligned(16))) char ring[NS * STAGE];
+  __shared__ __attribute__((aligned(16))) char ring[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
@@ -412,7 +479,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   const LinearSlice slice = linear_slice(p, OpY::BK);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
-  int y_rd[YT ? RBW : 1], x_rd[XT ? NBW : 1];
+  int y_rd[YT ? RBW : 2], x_rd[XT ? NBW : 2];
   y.offsets(lane, wm, y_rd);
   x.offsets(lane, wn, x_rd);
   AccV acc[RBW][NBW];
@@ -427,26 +494,15 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
     y.issue_next(st, wave, live);
     x.issue_next(st + OpY::VECS * 16, wave, live);
   };
-  v4i ya[RBW], xa[NBW], yb[RBW], xb[NBW];   // the fragments of two steps
-  auto read = [&](int stage, v4i (&yf)[RBW], v4i (&xf)[NBW]) __attribute__((always_inline)) {
+  v4i ya[RBW], xa[NBW], yb[RBW], xb[NBW];   // the fragments of two halves
+  auto read = [&](int stage, int half, v4i (&yf)[RBW], v4i (&xf)[NBW]) __attribute__((always_inline)) {
     const char *st = ring + stage * STAGE;
 #pragma unroll
-    for (int nb = 0; nb < NBW; ++nb) xf[nb] = OpX::fragment(st + OpY::VECS * 16, x_rd, 0, nb);
+    for (int nb = 0; nb < NBW; ++nb) xf[nb] = OpX::fragment(st + OpY::VECS * 16, x_rd, half, nb);
 #pragma unroll
-    for (int rb = 0; rb < RBW; ++rb) yf[rb] = OpY::fragment(st, y_rd, 0, rb);
+    for (int rb = 0; rb < RBW; ++rb) yf[rb] = OpY::fragment(st, y_rd, half, rb);
   };
-  for (int s = 0; s < NS; ++s) issue(s, s);
-  wait_vmcnt<(NS - 1) * PER>();
-  lds_barrier();
-  read(0, ya, xa);
-  int cs = 0;
-  auto phase = [&](int s, v4i (&yc)[RBW], v4i (&xc)[NBW], v4i (&yn)[RBW], v4i (&xn)[NBW]) __attribute__((always_inline)) {
-    wait_vmcnt<(NS - 2) * PER>();
-    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): the fragments of step s are in registers
-    lds_barrier();
-    issue(s + NS, cs);
-    cs = cs + 1 == NS ? 0 : cs + 1;
-    read(cs, yn, xn);
+  auto products = [&](v4i (&yc)[RBW], v4i (&xc)[NBW]) __attribute__((always_inline)) {
 #pragma unroll
     for (int rb = 0; rb < RBW; ++rb)
 #pragma unroll
@@ -461,16 +517,26 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
     }
     __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
   };
-  int s = 0;
-  for (; s + 1 < slice.steps; s += 2) {
-    phase(s, ya, xa, yb, xb);
-    phase(s + 1, yb, xb, ya, xa);
+  issue(0, 0);
+  issue(1, 1);
+  wait_vmcnt<PER>();
+  lds_barrier();
+  read(0, 0, ya, xa);
+  for (int s = 0; s < slice.steps; ++s) {
+    const int st = s & 1;
+    read(st, 1, yb, xb);
+    products(ya, xa);
+    wait_vmcnt<0>();                        // the next step is there,
+    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): all of this one is in registers
+    lds_barrier();
+    issue(s + 2, st);
+    read(st ^ 1, 0, ya, xa);
+    products(yb, xb);
   }
-  if (s < slice.steps) phase(s, ya, xa, yb, xb);
   wait_vmcnt<0>();
   __builtin_amdgcn_s_waitcnt(0xC07F);
   lds_barrier();
-  constexpr int SHARE = NS * STAGE / (WM * WN);
+  constexpr int SHARE = 2 * STAGE / (WM * WN);
   linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE);
 }
 
@@ -533,25 +599,26 @@ __global__ __launch_bounds__(W * 64) void linear_few_kernel(const LinearParams p
   wait_vmcnt<0>();
   __builtin_amdgcn_s_waitcnt(0xC07F);
   asm volatile("" ::: "memory");
-  // every wave parks its sums in its own ring: [row][column], 16 of each per block
+  // every wave parks its sums in its own ring: [row][column], 16 of those
   const int i = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int b = 0; b < MB; ++b) reinterpret_cast<AccV *>(&ring[wave][0])[(b * 16 + i) * 4 + q] = acc[b];
   __syncthreads();
   for (int t = tid; t < MB * 32; t += W * 64) {
-    const int m = t >> 1, half = t & 1;
-    if (m >= p.m || n0 + half * 8 >= p.n) continue;
-    AccV a = reinterpret_cast<const AccV *>(&ring[0][0])[m * 4 + half * 2], b = reinterpret_cast<const AccV *>(&ring[0][0])[m * 4 + half * 2 + 1];
+    const int m = t >> 1, piece = t & 1, n = n0 + piece * 8;
+    if (m >= p.m || n >= p.n) continue;
+    const int at = m * 4 + piece * 2;
+    AccV a = reinterpret_cast<const AccV *>(&ring[0][0])[at], b = reinterpret_cast<const AccV *>(&ring[0][0])[at + 1];
 #pragma unroll
     for (int w = 1; w < W; ++w) {
-      a += reinterpret_cast<const AccV *>(&ring[w][0])[m * 4 + half * 2];
-      b += reinterpret_cast<const AccV *>(&ring[w][0])[m * 4 + half * 2 + 1];
+      a += reinterpret_cast<const AccV *>(&ring[w][0])[at];
+      b += reinterpret_cast<const AccV *>(&ring[w][0])[at + 1];
     }
     float v[8], bias[8], scale[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (float)a[e], v[4 + e] = (float)b[e];
-    linear_columns<OUT, S8OP>(p, n0 + half * 8, bias, scale);
-    linear_finish8<OUT, S8OP, false>(p, m, n0 + half * 8, v, bias, scale);
+    linear_columns<OUT, S8OP>(p, n, bias, scale);
+    linear_finish8<OUT, S8OP, false>(p, m, n, v, bias, scale);
   }
 }
 

@@ -12,25 +12,49 @@ namespace cummhip {
 
 #ifdef CUMM_LINEAR_HOST
 
+// Which kernel and how many slices: the least estimated time, in us on 256 CUs.  The figures are fitted (non-negative least
+// squares of the relative error, 12 % on average) to 26 k timings of 2100 random products of all three layouts, bf16: m to
+// 120000, n to 16384, k to 100000.  With them the choice is 4 % slower than the fastest of every kernel and number of
+// slices tried.  R: workgroups per CU, rounded up while there are one or two, as they are beyond; steps of 64 k.
+//   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
+// 64 x 64 in 2 x 2 x 2 waves and 64 x 128 in 2 x 4, three stages; 128 x 128 and 256 x 256 through registers.  Few
+// rows (17 to 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
+// (31 x 2376 x 72 4.8 us against 14.1 in eight slices), above them while one round of workgroups does (60 x 5256 x 15680
+// 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 57 us in 64 slices of
+// one large tile each, 111 in 16 of the small); the large tile from about one per CU on (4096^3 103 us against 125).
+struct TileFigures {
+  double launch, turn, step, operands, partial, join;
+};
+constexpr TileFigures kTiles[4][3] = {
+    {{0, 3.604, 0.2456, 0.02245, 0.755, 2.368}, {0, 2.408, 0.2451, 5.555e-05, 0.6614, 1.46}, {4.485, 0.7715, 0.2747, 0, 0.3164, 1.563}},      // 64 x 64
+    {{3.747, 0, 0.3336, 0.02478, 0.6734, 2.261}, {0, 2.534, 0.3085, 0.04972, 0.6238, 0.568}, {4.945, 1.083, 0.3618, 0.0278, 0.268, 1.744}},      // 64 x 128
+    {{4.519, 0, 0.4515, 0.1012, 0.6342, 1.735}, {0, 3.642, 0.4106, 0.02338, 0.4841, 0}, {6.664, 1.293, 0.5791, 0.02827, 0.2903, 0}},      // 128 x 128
+    {{7.887, 0, 1.148, 0.03461, 0.4533, 1.027}, {2.338, 4.53, 1.418, 0.02914, 0.3328, 0}, {2.338, 4.53, 1.418, 0.02914, 0.3328, 0}},      // 256 x 256
+};
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
-  if (layout == kResult && m <= 64) return {kTileFew, 1};
-  const auto tiles = [&](int tm, int tn) { return ((m + tm - 1) / tm) * (int64_t)((n + tn - 1) / tn); };
-  const double kd = (double)k;
+  if (layout == kResult && m <= 16) return {kTileFew, 1};
   LinearPlan best = {kTile64, 1};
   double least = 1e300;
+  const double operands = ((double)m * k + (double)n * k) * 2e-6, sums = (double)m * n * 4e-6;
+  if (layout == kResult && m <= 64) {
+    const bool two = m <= 32;      // blocks of 16 rows: two workgroups fit a CU, else one
+    const double rounds = (double)(((n + 15) / 16 + (two ? 511 : 255)) / (two ? 512 : 256)), steps = (double)((k + 255) / 256);
+    least = two ? 0.9518 + rounds * (1.93 + 0.2101 * steps) : 1.342 + rounds * (1.937 + 0.2799 * steps);
+    best = {kTileFew, 1};
+  }
+  constexpr int kShape[4][3] = {{64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {256, 256, kTile256}};
   for (int slices = 1; slices <= 256; slices *= 2) {
-    if (slices > 1 && k / slices < 256) break;
-    const double ks = kd / slices;
-    const double join = slices == 1 ? 0.0 : 4.0 + (double)m * n * 4.0 * (2.0 * slices) / 4e6;
-    const auto per_cu = [&](int tm, int tn) { return (double)((tiles(tm, tn) * slices + 255) / 256); };
-    const auto consider = [&](int tile, double us) {
-      if (us + join < least) least = us + join, best = {tile, slices};
-    };
-    const double n64 = per_cu(64, 64), n128 = per_cu(128, 128), n256 = per_cu(256, 256);
-    consider(kTile64, n64 == 1 ? 3.7 + 0.0040 * ks : (n64 == 2 ? 4.9 + 0.0063 * ks : 2.4 + n64 * (1.12 + 0.0031 * ks)));
-    if (n128 == 1) consider(kTile128Deep, std::max(9.4, 7.0 + 0.0072 * ks));
-    else consider(kTile128, n128 == 2 ? 8.2 + 0.0122 * ks : n128 * (3.9 + 0.0077 * ks));
-    consider(kTile256, std::max(2.0 + n256 * (14.8 + 0.0235 * ks), 8.5 + 0.0255 * n256 * ks));
+    if (slices > 1 && k / slices < 128) break;
+    const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
+    for (int t = 0; t < 4; ++t) {
+      const double wgs = (double)((m + kShape[t][0] - 1) / kShape[t][0]) * (double)((n + kShape[t][1] - 1) / kShape[t][1]) * slices;
+      const int regime = wgs <= 256 ? 0 : (wgs <= 512 ? 1 : 2);
+      const double rounds = regime < 2 ? regime + 1.0 : (t == 3 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
+      const TileFigures &f = kTiles[t][regime];
+      const double us = f.launch + rounds * (f.turn + f.step * steps) + f.operands * (operands + (slices == 1 ? sums / 2 : 0.0)) +
+                        (slices == 1 ? 0.0 : f.partial * sums * slices + f.join);
+      if (us < least) least = us, best = {kShape[t][2], slices};
+    }
   }
   return best;
 }
@@ -66,11 +90,12 @@ static hipError_t ring(const LinearParams &p, hipStream_t s) {
                      dim3(WM * WN * WK * 64), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
-template <class T, class OUT, bool XT, bool YT>
+template <class T, class OUT, int RBW, int NBW, bool XT, bool YT>
 static hipError_t pipe(const LinearParams &p, hipStream_t s) {
-  if (!counted_waits_hold<linear_pipe_kernel<T, OUT, 2, 4, 8, 4, 4, XT, YT>>()) return hipErrorNotSupported;
-  const int tiles_m = (int)((p.m + 255) / 256), tiles_n = (p.n + 255) / 256;
-  hipLaunchKernelGGL((linear_pipe_kernel<T, OUT, 2, 4, 8, 4, 4, XT, YT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(512), 0, s, p,
+  constexpr int TM = 2 * RBW * 16, TN = 4 * NBW * 16;
+  if (!counted_waits_hold<linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, XT, YT>>()) return hipErrorNotSupported;
+  const int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (p.n + TN - 1) / TN;
+  hipLaunchKernelGGL((linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, XT, YT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(512), 0, s, p,
                      tiles_m, tiles_n);
   return hipGetLastError();
 }
@@ -87,15 +112,17 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
   switch (plan.tile) {
   case kTileFew:
     if constexpr (!XT && !YT) {
-      if (p.m <= 16) return few<T, OUT, 4, 1, 2, 3>(p, s);
+      // (two waves where there are several workgroups per CU, else eight: 1 x 4096 x 16384 bf16 26.9 us against 28.5,
+      // 4 x 8192 x 256 13.8 against 6.7)
+      if (p.m <= 16) return p.n >= 8192 ? few<T, OUT, 2, 1, 2, 4>(p, s) : few<T, OUT, 8, 1, 2, 3>(p, s);
       if (p.m <= 32) return few<T, OUT, 4, 2, 2, 3>(p, s);
       if (p.m <= 64) return few<T, OUT, 4, 4, 2, 3>(p, s);
     }
     return e;
   case kTile64: e = ring<T, OUT, 2, 2, 2, 2, 2, 2, 3, XT, YT>(p, s); break;
-  case kTile128: e = ring<T, OUT, 2, 4, 1, 4, 2, 2, 2, XT, YT>(p, s); break;
-  case kTile128Deep: e = ring<T, OUT, 2, 4, 1, 4, 2, 2, 4, XT, YT>(p, s); break;
-  case kTile256: e = pipe<T, OUT, XT, YT>(p, s); break;
+  case kTile64x128: e = ring<T, OUT, 2, 4, 1, 2, 2, 2, 3, XT, YT>(p, s); break;
+  case kTile128: e = pipe<T, OUT, 4, 2, XT, YT>(p, s); break;
+  case kTile256: e = pipe<T, OUT, 8, 4, XT, YT>(p, s); break;
   }
   return e == hipSuccess ? join<T, OUT>(p, s) : e;
 }
