@@ -14,7 +14,7 @@ struct LinearPlan {
   int tile;      // kTile*
   int slices;
 };
-enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile256 = 4 };
+enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5 };
 // k in units of two bytes
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k);
 // bytes of the slices' sums (0 = one slice)
@@ -25,8 +25,7 @@ hipError_t launch_linear_f16(LinearLayout layout, const LinearPlan &plan, const 
 hipError_t launch_linear_bf16(LinearLayout layout, const LinearPlan &plan, const LinearParams &p, hipStream_t s);
 // 8-bit operands, output f16 or bf16 (layout kResult)
 hipError_t launch_linear_s8(bool bf16, const LinearPlan &plan, const LinearParams &p, hipStream_t s);
-// rows x cols elements of 1 or 2 bytes to rows of to_ld bytes (a multiple of 16), zeros behind them
-hipError_t launch_linear_repack(void *to, const void *from, int64_t rows, int64_t cols, int64_t ld, int64_t to_ld, int elem_bytes, hipStream_t s);
+hipError_t launch_linear_repack(LinearRepack p, int elem_bytes, hipStream_t s);      // (pieces and wgs are filled in)
 
 struct LinearGateParams {
   const void *grad;        // [rows, n]

@@ -43,8 +43,11 @@ struct Operand {
   void place(Workspace &w) {
     if (!direct()) copy = w.take(rows * pitch());
   }
-  hipError_t fill(hipStream_t s) const { return direct() ? hipSuccess : launch_linear_repack(copy, from, rows, cols, ld, pitch(), bytes, s); }
+  LinearRepack::One repack() const { return direct() ? LinearRepack::One{} : LinearRepack::One{copy, from, rows, cols, ld, pitch(), 0, 0}; }
 };
+hipError_t fill(const Operand &a, const Operand &b, hipStream_t s) {
+  return a.direct() && b.direct() ? hipSuccess : launch_linear_repack(LinearRepack{{a.repack(), b.repack()}}, a.bytes, s);
+}
 
 bool tiles_fit(int64_t m, int64_t n) { return (m + 63) / 64 * ((n + 63) / 64) <= 0x7fffffff; }
 
@@ -111,7 +114,7 @@ const char *linear_grad_checked(const CummHipLinearGradArgs &a) {
 }
 
 struct LinearGradCall {
-  Operand x, weight;
+  Operand x = {nullptr, 0, 0, 0, 2}, weight = x;      // (none, and so in place)
   LinearGateParams gate = {};
   bool gated;              // a launch that writes dz, or the bias sums, or both
   const void *dz;
@@ -217,8 +220,7 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
   const LinearCall call(*a, w);
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipError_t e = call.x.fill(s);
-  if (e == hipSuccess) e = call.weight.fill(s);
+  const hipError_t e = fill(call.x, call.weight, s);
   if (e != hipSuccess) return launched(e);
   LinearParams p = {};
   p.X = call.weight.at();
@@ -267,8 +269,8 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
   const bool bf16 = a->dtype == CUMM_HIP_BF16;
   hipError_t e = call.gated ? launch_linear_gate(call.gate, call.ldz, a->grad_bias, bf16, s) : hipSuccess;
+  if (e == hipSuccess) e = fill(call.x, call.weight, s);
   if (e == hipSuccess && a->grad_x) {
-    e = call.weight.fill(s);
     LinearParams p = {};
     p.Y = call.dz;
     p.ldy = call.ldz * 2;
@@ -281,10 +283,9 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
     p.ldo = a->k;
     p.partial = call.partial_x;
     p.slices = call.plan_x.slices;
-    if (e == hipSuccess) e = launch_two_byte(a->dtype, kGradInput, call.plan_x, p, s);
+    e = launch_two_byte(a->dtype, kGradInput, call.plan_x, p, s);
   }
   if (e == hipSuccess && a->grad_weight) {
-    e = call.x.fill(s);
     LinearParams p = {};
     p.Y = call.dz;
     p.ldy = call.ldz * 2;
@@ -297,7 +298,7 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
     p.ldo = a->k;
     p.partial = call.partial_w;
     p.slices = call.plan_w.slices;
-    if (e == hipSuccess) e = launch_two_byte(a->dtype, kGradWeight, call.plan_w, p, s);
+    e = launch_two_byte(a->dtype, kGradWeight, call.plan_w, p, s);
   }
   return launched(e);
 }

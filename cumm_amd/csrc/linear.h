@@ -179,10 +179,10 @@ __device__ __forceinline__ void linear_finish8(const LinearParams &p, int64_t m,
 // back as eight consecutive columns a lane: whole lines of 64 or 128 bytes per row and store, and a loop over rows instead
 // of an epilogue written out for every accumulator, which needs more registers than the large tile leaves.  Rows are
 // [row][16 or 8 units of four columns], units permuted by the row: neither side meets a bank twice.  The residual and the
-// rows' scales are fetched a group of rows ahead (row by row, a round trip to memory each, 8192 x 4096 x 4096 with a
-// residual takes 235 us, 25 more than without; so 218).
+// rows' scales are fetched a group of rows ahead.
 template <class OUT, bool S8, int RBW, int NBW, bool XT, bool NT, int BYTES, class AccV>
-__device__ __forceinline__ void linear_epilogue(const LinearParams &p, const AccV (&acc)[RBW][NBW], int64_t m_wave, int n_wave, int lane, char *lds) {
+__device__ __forceinline__ void linear_epilogue(const LinearParams &p, const AccV (&acc)[RBW][NBW], int64_t m_wave, int n_wave, int lane, char *lds,
+                                                int slice) {
   constexpr int UNITS = NBW * 4, PIECES = NBW * 2, ROWS = 64 / PIECES;      // ROWS at a time
   constexpr int FIT = BYTES / (NBW * 1024), CHUNK = FIT >= RBW ? RBW : (FIT >= 4 ? 4 : (FIT >= 2 ? 2 : 1));
   constexpr int TIMES = CHUNK * 16 / ROWS, GROUP = TIMES < 4 ? TIMES : 4, GROUPS = TIMES / GROUP, ALL = RBW / CHUNK * GROUPS;
@@ -208,7 +208,7 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const Acc
   };
   if (p.partial != nullptr) {      // 32-bit sums of this slice (8-bit operands: whole numbers)
     const int64_t n8 = (p.n + 7) & ~7;
-    v4i *to = reinterpret_cast<v4i *>(p.partial) + ((int64_t)blockIdx.y * p.m * n8 + n) / 4;
+    v4i *to = reinterpret_cast<v4i *>(p.partial) + ((int64_t)slice * p.m * n8 + n) / 4;
 #pragma unroll
     for (int chunk = 0; chunk < RBW / CHUNK; ++chunk) {
       park(chunk);
@@ -272,7 +272,10 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const Acc
           Piece<OUT> out;
           out.round(t);
           const int64_t m = m0 + j * ROWS;
-          if (m < p.m && in_n) out.template store<NT>(base, m * ld + n, count);
+          if (m < p.m && in_n) {
+            if (NT && ld % 64 == 0) out.template store<true>(base, m * ld + n, count);
+            else out.store(base, m * ld + n, count);
+          }
         }
       };
       if (p.pre != nullptr) store(p.pre, p.ldp);
@@ -294,9 +297,8 @@ template <int ROWS, int KS, int WAVES, bool TR, int SLAB_BLOCKS, bool WIDE_ORDER
 struct LinearOperand : DenseOperand<ROWS, KS, WAVES, TR, SLAB_BLOCKS, WIDE_ORDER> {
   using Base = DenseOperand<ROWS, KS, WAVES, TR, SLAB_BLOCKS, WIDE_ORDER>;
   using Base::voff;
-  using Base::kpos;
   uint64_t at;       // where the next step begins
-  int64_t left;      // k from there on
+  int left;          // k from there on
   uint64_t step;     // bytes
 
   // rows first .. first + ROWS of `count`, from step `s0` on
@@ -307,45 +309,54 @@ struct LinearOperand : DenseOperand<ROWS, KS, WAVES, TR, SLAB_BLOCKS, WIDE_ORDER
       const int slot = (wave * Base::IP + t) * 64 + lane;
       if constexpr (TR) {
         const int e = slot / Base::CPR, c = (slot % Base::CPR) ^ Base::swap_tr(e);
-        kpos[t] = e;
         voff[t] = c * 8 < rows_here ? (uint32_t)(e * ld) + (uint32_t)c * 16u : Base::kOob;
       } else {
         const int rho = slot / Base::LPR, c = (slot % Base::LPR) ^ Base::swap_kc(rho);
         const int i = rho & 15, nb = (rho >> 4) % SLAB_BLOCKS, slab = rho / (16 * SLAB_BLOCKS);
         const int row = WIDE_ORDER ? slab * (16 * SLAB_BLOCKS) + (nb >> 1) * 32 + (i >> 2) * 8 + (nb & 1) * 4 + (i & 3) : rho;
-        kpos[t] = c * 8;
         voff[t] = row < rows_here ? (uint32_t)(row * ld) + (uint32_t)c * 16u : Base::kOob;
       }
     }
     step = (uint64_t)(TR ? (int64_t)Base::BK * ld : (int64_t)Base::BK * 2);
     at = (uint64_t)ptr + (uint64_t)(TR ? first * 2 : first * ld) + (uint64_t)s0 * step;
-    left = k - s0 * Base::BK;
+    left = (int)(k - s0 * Base::BK);
   }
-  // the next step, into the stage at `lds`; one that is not live is zeros, without traffic
-  __device__ __forceinline__ void issue_next(uint32_t lds, int wave, bool live) {
-    const v4i rsrc = {(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), live ? 0x7fffffff : 0, 0x00020000};
-    if (left >= Base::BK) {
+  // The next step, into the stage at `lds_at`; one that is not live is zeros, without traffic.  The last one takes the
+  // chunks that lie behind the end of k out of the offsets, for good: a look per step, not one per load (which the
+  // large tile takes 776 us for at 8192^3 instead of 759).
+  v4i rsrc;
+  uint32_t lds;
+  __device__ __forceinline__ void aim(uint32_t lds_at, int wave, int lane, bool live) {
+    rsrc = v4i{(int)(uint32_t)at, (int)((uint32_t)(at >> 32) & 0xffffu), live ? 0x7fffffff : 0, 0x00020000};
+    lds = lds_at + wave * Base::IP * 1024;
+    if (left < Base::BK) {
 #pragma unroll
-      for (int t = 0; t < Base::IP; ++t) dma_b128(rsrc, lds + (wave * Base::IP + t) * 1024, voff[t], 0u);
-    } else {
-      const int here = left < 0 ? 0 : (int)left;
-#pragma unroll
-      for (int t = 0; t < Base::IP; ++t) dma_b128(rsrc, lds + (wave * Base::IP + t) * 1024, kpos[t] < here ? voff[t] : Base::kOob, 0u);
+      for (int t = 0; t < Base::IP; ++t) {
+        const int slot = (wave * Base::IP + t) * 64 + lane;
+        const int first_k = TR ? slot / Base::CPR : ((slot % Base::LPR) ^ Base::swap_kc(slot / Base::LPR)) * 8;
+        voff[t] = first_k < left ? voff[t] : Base::kOob;
+      }
     }
     skip(1);
   }
+  __device__ __forceinline__ void issue_one(int t) const { dma_b128(rsrc, lds + t * 1024, voff[t], 0u); }
+  __device__ __forceinline__ void issue_next(uint32_t lds_at, int wave, int lane, bool live) {
+    aim(lds_at, wave, lane, live);
+#pragma unroll
+    for (int t = 0; t < Base::IP; ++t) issue_one(t);
+  }
   __device__ __forceinline__ void skip(int steps) {
     at += step * (uint64_t)steps;
-    left -= (int64_t)steps * Base::BK;
+    left -= steps * Base::BK;
   }
 };
 
-// The steps of slice blockIdx.y: whole steps, the last slice takes what is left
+// The steps of a slice: whole steps, the last slice takes what is left
 struct LinearSlice {
   int first, steps;
 };
-__device__ __forceinline__ LinearSlice linear_slice(const LinearParams &p, int step) {
-  const int all = (int)((p.k + step - 1) / step), per = (all + p.slices - 1) / p.slices, first = (int)blockIdx.y * per;
+__device__ __forceinline__ LinearSlice linear_slice(const LinearParams &p, int step, int slice) {
+  const int all = (int)((p.k + step - 1) / step), per = (all + p.slices - 1) / p.slices, first = slice * per;
   const int end = first + per < all ? first + per : all;
   return {first, end > first ? end - first : 0};
 }
@@ -374,7 +385,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   const int n0 = tile_n * TN;
   OpY y;
   OpX x;
-  const LinearSlice slice = linear_slice(p, OpY::BK);
+  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
   int y_rd[YT ? RBW : KW], x_rd[XT ? NBW : KW];
@@ -389,8 +400,8 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   auto issue = [&](int s, int stage) __attribute__((always_inline)) {
     const bool live = s < slice.steps;
     const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
-    y.issue_next(st, wave, live);
-    x.issue_next(st + OpY::VECS * 16, wave, live);
+    y.issue_next(st, wave, lane, live);
+    x.issue_next(st + OpY::VECS * 16, wave, lane, live);
   };
   for (int s = 0; s < L; ++s) issue(s, s);
   int cs = 0, ls = L;
@@ -422,7 +433,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   lds_barrier();                          // and so has every other
   constexpr int SHARE = NS * STAGE / (WM * WN * WK);
   if constexpr (WK == 1) {
-    linear_epilogue<OUT, S8OP, RBW, NBW, XT, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE);
+    linear_epilogue<OUT, S8OP, RBW, NBW, XT, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
   } else {
     // each group finishes its share of the row blocks: it adds up all groups' sums of them, in group order
     constexpr int RO = RBW / WK;
@@ -446,17 +457,16 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
       }
     __syncthreads();
     linear_epilogue<OUT, S8OP, RO, NBW, XT, false, SHARE>(p, own, m0 + wm * (RBW * 16) + wk * RO * 16, n0 + wn * (NBW * 16), lane,
-                                                          ring + wave * SHARE);
+                                                          ring + wave * SHARE, (int)blockIdx.y);
   }
 }
 
-// ---- the large tile, its fragments double-buffered in registers: while the products of one half of a step (32 k) run on
-// one set, those of the next half are read into the other.  A step is 64 k, so that a row's share of it is a whole line
-// of 128 bytes (with 32 k every line is asked for twice: 8192 x 4096 x 4096 250 us instead of 210), and there are two
-// stages: the loads of step s + 2 begin when the second half of step s is in registers, and have a whole step's products,
-// 2048 clocks of the matrix cores, to arrive.  Without the wait for them the time is the same (204 against 204), without
-// the loads it is 172: what is left of them is their traffic and its power, not their latency.
-template <class T, class OUT, int WM, int WN, int RBW, int NBW, bool XT, bool YT>
+// ---- fragments double-buffered in registers: while the products of one half of a step (32 k) run on one set, those of
+// the next half are read into the other.  A step is 64 k, so that a row's share of it is a whole line of 128 bytes (with
+// 32 k every line is asked for twice: 8192 x 4096 x 4096 in tiles of 256 250 us instead of 210), and there are two
+// stages: the loads of step s + 2 begin when the second half of step s is in registers.  Tiles of 128 x 128, two
+// workgroups per CU, one of which loads, waits or stores while the other multiplies.
+template <class T, class OUT, int WM, int WN, int RBW, int NBW, int NS, bool XT, bool YT>
 __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearParams p, int tiles_m, int tiles_n) {
   using E = Elem<T>;
   using AccV = typename E::AccV;
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   using OpX = LinearOperand<TN, 2, WM * WN, XT, NBW, !XT>;
   constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
   constexpr int PER = OpY::IP + OpX::IP;
-  __shared__ __attribute__((aligned(16))) char ring[2 * STAGE];
+  __shared__ __attribute__((aligned(16))) char ring[NS * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   const int n0 = tile_n * TN;
   OpY y;
   OpX x;
-  const LinearSlice slice = linear_slice(p, OpY::BK);
+  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
   int y_rd[YT ? RBW : 2], x_rd[XT ? NBW : 2];
@@ -491,8 +501,8 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   auto issue = [&](int s, int stage) __attribute__((always_inline)) {
     const bool live = s < slice.steps;
     const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
-    y.issue_next(st, wave, live);
-    x.issue_next(st + OpY::VECS * 16, wave, live);
+    y.issue_next(st, wave, lane, live);
+    x.issue_next(st + OpY::VECS * 16, wave, lane, live);
   };
   v4i ya[RBW], xa[NBW], yb[RBW], xb[NBW];   // the fragments of two halves
   auto read = [&](int stage, int half, v4i (&yf)[RBW], v4i (&xf)[NBW]) __attribute__((always_inline)) {
@@ -517,27 +527,123 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
     }
     __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
   };
-  issue(0, 0);
-  issue(1, 1);
-  wait_vmcnt<PER>();
+  for (int s = 0; s < NS; ++s) issue(s, s);
+  wait_vmcnt<(NS - 1) * PER>();
   lds_barrier();
   read(0, 0, ya, xa);
+  int st = 0;
   for (int s = 0; s < slice.steps; ++s) {
-    const int st = s & 1;
+    const int after = st + 1 == NS ? 0 : st + 1;
     read(st, 1, yb, xb);
     products(ya, xa);
-    wait_vmcnt<0>();                        // the next step is there,
+    wait_vmcnt<(NS - 2) * PER>();           // the next step is there,
     __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): all of this one is in registers
     lds_barrier();
-    issue(s + 2, st);
-    read(st ^ 1, 0, ya, xa);
+    issue(s + NS, st);
+    read(after, 0, ya, xa);
     products(yb, xb);
+    st = after;
   }
   wait_vmcnt<0>();
   __builtin_amdgcn_s_waitcnt(0xC07F);
   lds_barrier();
-  constexpr int SHARE = 2 * STAGE / (WM * WN);
-  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE);
+  constexpr int SHARE = NS * STAGE / (WM * WN);
+  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
+}
+
+// ---- the large tile: the same step, with loads and fragment reads dealt out among the products, a load per row block (all
+// eight at once hold a wave up until the address unit, 64 bytes per clock, has taken the 64 KB of all waves: 8192 x 4096 x
+// 4096 215 us, so 210), and the half of the products that loads at raised priority (207).  8192^3 bf16: 735 us, 1.5
+// PFLOP/s, the matrix cores busy 78 % of the time at 1.82 GHz, the chip's limit of power (on zeros, without loads, it
+// holds 2.42).  One workgroup per CU that goes on to the next tile, whose first steps it loads during the epilogue, takes 780.
+template <class T, class OUT, bool XT, bool YT>
+__global__ __launch_bounds__(512) void linear_large_kernel(const LinearParams p, int tiles_m, int tiles_n) {
+  using E = Elem<T>;
+  using AccV = typename E::AccV;
+  constexpr bool S8OP = E::kBytes == 1;
+  static_assert(!S8OP || (!XT && !YT), "8-bit operands are contiguous along k");
+  constexpr int WN = 4, RBW = 8, NBW = 4;      // 2 x 4 waves of 128 x 64
+  using OpY = LinearOperand<256, 2, 8, YT, RBW, false>;
+  using OpX = LinearOperand<256, 2, 8, XT, NBW, !XT>;
+  constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
+  constexpr int PER = OpY::IP + OpX::IP;
+  static_assert(PER == RBW, "a load per row block");
+  __shared__ __attribute__((aligned(16))) char ring[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int tile_m, tile_n;
+  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int64_t m0 = (int64_t)tile_m * 256;
+  const int n0 = tile_n * 256;
+  OpY y;
+  OpX x;
+  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
+  x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
+  int y_rd[YT ? RBW : 2], x_rd[XT ? NBW : 2];
+  y.offsets(lane, wm, y_rd);
+  x.offsets(lane, wn, x_rd);
+  AccV acc[RBW][NBW];
+#pragma unroll
+  for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = AccV{0, 0, 0, 0};
+  const uint32_t ring_at = lds_addr(ring);
+  auto aim = [&](int s, int stage) __attribute__((always_inline)) {
+    const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
+    y.aim(st, wave, lane, s < slice.steps);
+    x.aim(st + OpY::VECS * 16, wave, lane, s < slice.steps);
+  };
+  auto issue_one = [&](int t) __attribute__((always_inline)) {
+    if (t < OpY::IP) y.issue_one(t);
+    else x.issue_one(t - OpY::IP);
+  };
+  v4i ya[RBW], xa[NBW], yb[RBW], xb[NBW];   // the fragments of two halves
+  // the products of one half, the reads of the next one (of `stage`) and, with LOADS, those that were aimed in between
+  auto half = [&](auto loads, v4i (&yc)[RBW], v4i (&xc)[NBW], int stage, int next, v4i (&yn)[RBW], v4i (&xn)[NBW]) __attribute__((always_inline)) {
+    const char *st = ring + stage * STAGE;
+#pragma unroll
+    for (int rb = 0; rb < RBW; ++rb) {
+#pragma unroll
+      for (int i = 0; i < RBW + NBW; ++i) {
+        if (i * RBW / (RBW + NBW) != rb) continue;
+        if (i < NBW) xn[i] = OpX::fragment(st + OpY::VECS * 16, x_rd, next, i);
+        else yn[i - NBW] = OpY::fragment(st, y_rd, next, i - NBW);
+      }
+      if constexpr (decltype(loads)::value) issue_one(rb);
+#pragma unroll
+      for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = E::mfma(xc[nb], yc[rb], acc[rb][nb]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    aim(s, s);
+#pragma unroll
+    for (int t = 0; t < PER; ++t) issue_one(t);
+  }
+  wait_vmcnt<PER>();
+  lds_barrier();
+#pragma unroll
+  for (int nb = 0; nb < NBW; ++nb) xa[nb] = OpX::fragment(ring + OpY::VECS * 16, x_rd, 0, nb);
+#pragma unroll
+  for (int rb = 0; rb < RBW; ++rb) ya[rb] = OpY::fragment(ring, y_rd, 0, rb);
+  for (int s = 0; s < slice.steps; ++s) {
+    const int st = s & 1;
+    half(std::false_type{}, ya, xa, st, 1, yb, xb);
+    wait_vmcnt<0>();                        // the next step is there,
+    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0): all of this one is in registers
+    lds_barrier();
+    __builtin_amdgcn_s_setprio(1);
+    aim(s + 2, st);
+    half(std::true_type{}, yb, xb, st ^ 1, 0, ya, xa);
+    __builtin_amdgcn_s_setprio(0);
+  }
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  lds_barrier();
+  constexpr int SHARE = 2 * STAGE / 8;
+  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
 }
 
 // ---- few rows: MB blocks of 16 of them, 16 columns per workgroup, the steps dealt out to its W waves.  What counts is the
@@ -570,8 +676,8 @@ __global__ __launch_bounds__(W * 64) void linear_few_kernel(const LinearParams p
   const uint32_t ring_at = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(&ring[wave][0]));
   auto issue = [&](int j, int stage) __attribute__((always_inline)) {
     const uint32_t st = ring_at + (uint32_t)__builtin_amdgcn_readfirstlane(stage * STAGE);
-    y.issue_next(st, 0, j < mine);
-    x.issue_next(st + OpY::VECS * 16, 0, j < mine);
+    y.issue_next(st, 0, lane, j < mine);
+    x.issue_next(st + OpY::VECS * 16, 0, lane, j < mine);
     y.skip(W - 1);      // (the other waves' steps)
     x.skip(W - 1);
   };
@@ -661,20 +767,36 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const LinearParams p) 
   linear_finish8<OUT, S8, false>(p, m, n, v, bias, scale);
 }
 
-// An operand whose rows do not lie on 16-byte borders, or end between them: a copy whose rows do, zeros behind their
-// ends.  thread = 16 bytes of a row of `to`, ES bytes an element
+// Operands whose rows do not lie on 16-byte borders, or end between them: copies whose rows do, zeros behind their
+// ends.  thread = 16 bytes of a row; both operands of a product in one launch (none: no rows).
+struct LinearRepack {
+  struct One {
+    void *to;
+    const void *from;
+    int64_t rows, cols, ld, to_ld;      // elements, to_ld bytes (a multiple of 16)
+    int64_t pieces, wgs;
+  } of[2];
+};
 template <int ES>
-__global__ __launch_bounds__(256) void linear_repack_kernel(v4i *to, const void *from, int64_t rows, int64_t cols, int64_t ld, int64_t pieces, int64_t to_ld) {
+__global__ __launch_bounds__(256) void linear_repack_kernel(const LinearRepack p) {
   using U = std::conditional_t<ES == 1, uint8_t, uint16_t>;
+  using At = std::conditional_t<ES == 1, v4i_any1, v4i_any>;
   constexpr int PER = 16 / ES;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * pieces; t += (int64_t)gridDim.x * 256) {
-    const int64_t r = t / pieces, c = (t - r * pieces) * PER;
-    const U *src = reinterpret_cast<const U *>(from) + r * ld + c;
+  const bool second = (int64_t)blockIdx.x >= p.of[0].wgs;
+  const LinearRepack::One &o = p.of[second];
+  const int64_t first = (int64_t)blockIdx.x - (second ? p.of[0].wgs : 0);
+  for (int64_t t = first * 256 + threadIdx.x; t < o.rows * o.pieces; t += o.wgs * 256) {
+    const int64_t r = t / o.pieces, c = (t - r * o.pieces) * PER;
+    const U *src = reinterpret_cast<const U *>(o.from) + r * o.ld + c;
     v4i v;
-    U *u = reinterpret_cast<U *>(&v);
+    if (c + PER <= o.cols) {
+      v = *reinterpret_cast<const At *>(src);
+    } else {
+      U *u = reinterpret_cast<U *>(&v);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) u[e] = c + e < cols ? src[e] : (U)0;
-    to[r * (to_ld / 16) + c / PER] = v;
+      for (int e = 0; e < PER; ++e) u[e] = c + e < o.cols ? src[e] : (U)0;
+    }
+    reinterpret_cast<v4i *>(o.to)[r * (o.to_ld / 16) + c / PER] = v;
   }
 }
 

@@ -13,23 +13,26 @@ namespace cummhip {
 #ifdef CUMM_LINEAR_HOST
 
 // Which kernel and how many slices: the least estimated time, in us on 256 CUs.  The figures are fitted (non-negative least
-// squares of the relative error, 12 % on average) to 26 k timings of 2100 random products of all three layouts, bf16: m to
+// squares of the relative error, 12 % on average) to 29 k timings of 2100 random products of all three layouts, bf16: m to
 // 120000, n to 16384, k to 100000.  With them the choice is 4 % slower than the fastest of every kernel and number of
-// slices tried.  R: workgroups per CU, rounded up while there are one or two, as they are beyond; steps of 64 k.
+// slices tried.  R: workgroups per CU, rounded up while there are one or two (one per CU: always), as they are beyond; steps
+// of 64 k.
 //   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
-// 64 x 64 in 2 x 2 x 2 waves and 64 x 128 in 2 x 4, three stages; 128 x 128 and 256 x 256 through registers.  Few
-// rows (17 to 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
+// 64 x 64 in 2 x 2 x 2 waves and 64 x 128 in 2 x 4, three stages; the others through registers.  Few rows (17 to
+// 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
 // (31 x 2376 x 72 4.8 us against 14.1 in eight slices), above them while one round of workgroups does (60 x 5256 x 15680
 // 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 57 us in 64 slices of
-// one large tile each, 111 in 16 of the small); the large tile from about one per CU on (4096^3 103 us against 125).
+// one large tile each, 111 in 16 of the small); 128 x 256 where the large tile leaves half of the CUs idle (4096 x 8192 x
+// 2048 123 us, 128 x 128 142, 256 x 256 186); the large tile from about one per CU on (4096^3 103 us against 125).
 struct TileFigures {
   double launch, turn, step, operands, partial, join;
 };
-constexpr TileFigures kTiles[4][3] = {
-    {{0, 3.604, 0.2456, 0.02245, 0.755, 2.368}, {0, 2.408, 0.2451, 5.555e-05, 0.6614, 1.46}, {4.485, 0.7715, 0.2747, 0, 0.3164, 1.563}},      // 64 x 64
-    {{3.747, 0, 0.3336, 0.02478, 0.6734, 2.261}, {0, 2.534, 0.3085, 0.04972, 0.6238, 0.568}, {4.945, 1.083, 0.3618, 0.0278, 0.268, 1.744}},      // 64 x 128
-    {{4.519, 0, 0.4515, 0.1012, 0.6342, 1.735}, {0, 3.642, 0.4106, 0.02338, 0.4841, 0}, {6.664, 1.293, 0.5791, 0.02827, 0.2903, 0}},      // 128 x 128
-    {{7.887, 0, 1.148, 0.03461, 0.4533, 1.027}, {2.338, 4.53, 1.418, 0.02914, 0.3328, 0}, {2.338, 4.53, 1.418, 0.02914, 0.3328, 0}},      // 256 x 256
+constexpr TileFigures kTiles[5][3] = {
+    {{0, 3.421, 0.221, 0.03681, 0.8072, 2.345}, {0, 2.285, 0.2482, 0, 0.6787, 1.389}, {4.212, 0.7239, 0.277, 0, 0.3323, 1.649}},      // 64 x 64
+    {{3.57, 0, 0.3104, 0.04129, 0.7229, 2.229}, {0, 2.476, 0.3057, 0.05074, 0.6454, 0.411}, {4.838, 1.048, 0.3628, 0.02501, 0.2659, 2.122}},      // 64 x 128
+    {{4.554, 0, 0.418, 0.0259, 0.6964, 1.825}, {0, 3.486, 0.4362, 0.01508, 0.4837, 0}, {6.421, 1.221, 0.5828, 0.02649, 0.2903, 0}},      // 128 x 128
+    {{0, 6.649, 0.6843, 0.03072, 0.5685, 0.8315}, {4.111, 4.333, 0.8235, 0.02194, 0.2804, 0}, {4.111, 4.333, 0.8235, 0.02194, 0.2804, 0}},      // 128 x 256
+    {{8.754, 0, 1.023, 0.04024, 0.4486, 0}, {1.944, 4.234, 1.359, 0.02885, 0.3361, 0}, {1.944, 4.234, 1.359, 0.02885, 0.3361, 0}},      // 256 x 256
 };
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
   if (layout == kResult && m <= 16) return {kTileFew, 1};
@@ -39,17 +42,17 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
   if (layout == kResult && m <= 64) {
     const bool two = m <= 32;      // blocks of 16 rows: two workgroups fit a CU, else one
     const double rounds = (double)(((n + 15) / 16 + (two ? 511 : 255)) / (two ? 512 : 256)), steps = (double)((k + 255) / 256);
-    least = two ? 0.9518 + rounds * (1.93 + 0.2101 * steps) : 1.342 + rounds * (1.937 + 0.2799 * steps);
+    least = two ? 0.8777 + rounds * (2.16 + 0.1743 * steps) : 1.415 + rounds * (2.016 + 0.2803 * steps);
     best = {kTileFew, 1};
   }
-  constexpr int kShape[4][3] = {{64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {256, 256, kTile256}};
+  constexpr int kShape[5][3] = {{64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
   for (int slices = 1; slices <= 256; slices *= 2) {
     if (slices > 1 && k / slices < 128) break;
     const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 5; ++t) {
       const double wgs = (double)((m + kShape[t][0] - 1) / kShape[t][0]) * (double)((n + kShape[t][1] - 1) / kShape[t][1]) * slices;
       const int regime = wgs <= 256 ? 0 : (wgs <= 512 ? 1 : 2);
-      const double rounds = regime < 2 ? regime + 1.0 : (t == 3 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
+      const double rounds = regime < 2 ? regime + 1.0 : (t >= 3 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
       const TileFigures &f = kTiles[t][regime];
       const double us = f.launch + rounds * (f.turn + f.step * steps) + f.operands * (operands + (slices == 1 ? sums / 2 : 0.0)) +
                         (slices == 1 ? 0.0 : f.partial * sums * slices + f.join);
@@ -59,12 +62,16 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
   return best;
 }
 
-hipError_t launch_linear_repack(void *to, const void *from, int64_t rows, int64_t cols, int64_t ld, int64_t to_ld, int elem_bytes, hipStream_t s) {
-  const int64_t pieces = (cols * elem_bytes + 15) / 16;
-  const int64_t wgs = std::min<int64_t>((rows * pieces + 255) / 256, 1 << 20);
+hipError_t launch_linear_repack(LinearRepack p, int elem_bytes, hipStream_t s) {
+  int64_t wgs = 0;
+  for (LinearRepack::One &o : p.of) {
+    o.pieces = (o.cols * elem_bytes + 15) / 16;
+    o.wgs = std::min<int64_t>((o.rows * o.pieces + 255) / 256, 1 << 20);
+    wgs += o.wgs;
+  }
   if (wgs == 0) return hipSuccess;
-  if (elem_bytes == 1) hipLaunchKernelGGL(linear_repack_kernel<1>, dim3((unsigned)wgs), dim3(256), 0, s, (v4i *)to, from, rows, cols, ld, pieces, to_ld);
-  else hipLaunchKernelGGL(linear_repack_kernel<2>, dim3((unsigned)wgs), dim3(256), 0, s, (v4i *)to, from, rows, cols, ld, pieces, to_ld);
+  if (elem_bytes == 1) hipLaunchKernelGGL(linear_repack_kernel<1>, dim3((unsigned)wgs), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(linear_repack_kernel<2>, dim3((unsigned)wgs), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -90,13 +97,20 @@ static hipError_t ring(const LinearParams &p, hipStream_t s) {
                      dim3(WM * WN * WK * 64), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
-template <class T, class OUT, int RBW, int NBW, bool XT, bool YT>
+template <class T, class OUT, int RBW, int NBW, int NS, bool XT, bool YT>
 static hipError_t pipe(const LinearParams &p, hipStream_t s) {
   constexpr int TM = 2 * RBW * 16, TN = 4 * NBW * 16;
-  if (!counted_waits_hold<linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, XT, YT>>()) return hipErrorNotSupported;
+  if (!counted_waits_hold<linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, NS, XT, YT>>()) return hipErrorNotSupported;
   const int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (p.n + TN - 1) / TN;
-  hipLaunchKernelGGL((linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, XT, YT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(512), 0, s, p,
+  hipLaunchKernelGGL((linear_pipe_kernel<T, OUT, 2, 4, RBW, NBW, NS, XT, YT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(512), 0, s, p,
                      tiles_m, tiles_n);
+  return hipGetLastError();
+}
+template <class T, class OUT, bool XT, bool YT>
+static hipError_t large(const LinearParams &p, hipStream_t s) {
+  if (!counted_waits_hold<linear_large_kernel<T, OUT, XT, YT>>()) return hipErrorNotSupported;
+  const int tiles_m = (int)((p.m + 255) / 256), tiles_n = (p.n + 255) / 256;
+  hipLaunchKernelGGL((linear_large_kernel<T, OUT, XT, YT>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(512), 0, s, p, tiles_m, tiles_n);
   return hipGetLastError();
 }
 template <class T, class OUT, int W, int MB, int KS, int NS>
@@ -121,8 +135,12 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
     return e;
   case kTile64: e = ring<T, OUT, 2, 2, 2, 2, 2, 2, 3, XT, YT>(p, s); break;
   case kTile64x128: e = ring<T, OUT, 2, 4, 1, 2, 2, 2, 3, XT, YT>(p, s); break;
-  case kTile128: e = pipe<T, OUT, 4, 2, XT, YT>(p, s); break;
-  case kTile256: e = pipe<T, OUT, 8, 4, XT, YT>(p, s); break;
+  case kTile128:      // (three stages where a CU has one workgroup: 2048^3 21.9 us against 24.9; two of two: 8192 x 1024 x 2048 39 against 48)
+    if (((p.m + 127) / 128) * ((p.n + 127) / 128) * p.slices <= 256) e = pipe<T, OUT, 4, 2, 3, XT, YT>(p, s);
+    else e = pipe<T, OUT, 4, 2, 2, XT, YT>(p, s);
+    break;
+  case kTile128x256: e = pipe<T, OUT, 4, 4, 3, XT, YT>(p, s); break;
+  case kTile256: e = large<T, OUT, XT, YT>(p, s); break;
   }
   return e == hipSuccess ? join<T, OUT>(p, s) : e;
 }

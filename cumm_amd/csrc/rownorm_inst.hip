@@ -502,15 +502,15 @@ hipError_t launch_norm_backward(const NormGradParams &p, bool bf16, hipStream_t 
   return bf16 ? norm_backward_of<BF16>(p, s) : norm_backward_of<F16>(p, s);
 }
 
-// A strip is 32 pieces of eight columns, fewer for narrow rows; blocks of rows so that there are some 2048 workgroups, of at
-// least 4 trips
+// A strip is 32 pieces of eight columns, fewer for narrow rows; blocks of rows so that there are some 1024 workgroups, of at
+// least one trip of 4 rows per thread
 void linear_gate_shape(int64_t rows, int n, int *shift, int *strips, int *blocks, int64_t *per) {
   const int pieces = (n + 7) / 8;
   *shift = 0;
   while (*shift < 5 && (1 << *shift) < pieces) ++*shift;
   *strips = (pieces + (1 << *shift) - 1) >> *shift;
   const int64_t trip = 4 * (256 >> *shift);
-  int64_t want = 2048 / *strips;
+  int64_t want = 1024 / *strips;
   if (want < 1) want = 1;
   int64_t rows_each = (rows + want - 1) / want;
   rows_each = (rows_each + trip - 1) / trip * trip;

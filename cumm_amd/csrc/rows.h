@@ -12,6 +12,7 @@ template <> struct Elem<F32> {
 };
 
 typedef int v4i_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int v4i_any1 __attribute__((ext_vector_type(4), aligned(1)));
 typedef int v4i_any4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
 
