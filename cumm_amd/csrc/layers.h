@@ -14,7 +14,7 @@ struct LinearPlan {
   int tile;      // kTile*
   int slices;
 };
-enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5 };
+enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5, kTile64Small = 6 };
 // k in units of two bytes
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k);
 // bytes of the slices' sums (0 = one slice)

@@ -49,17 +49,17 @@ constexpr float kGeluA = 2.30220819813f, kGeluB = 0.10294324038f;      // kLog2e
 __device__ __forceinline__ float logistic_of_exponent(float t) {      // 1 / (1 + 2^t)
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
-// Half of erfc(|z| / sqrt 2), the smaller tail of the normal distribution: Abramowitz and Stegun 7.1.26 (error of erf below
-// 1.5e-7), and e^(-z^2 / 2) beside it
+// The smaller tail of the normal distribution beyond |z|: Abramowitz and Stegun 26.2.17 (error below 7.5e-8), and
+// e^(-z^2 / 2) beside it
 __device__ __forceinline__ float normal_tail(float z, float *e) {
-  const float x = __builtin_fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
-  float poly = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  poly = __builtin_fmaf(poly, t, 1.421413741f);
-  poly = __builtin_fmaf(poly, t, -0.284496736f);
-  poly = __builtin_fmaf(poly, t, 0.254829592f);
-  *e = __builtin_amdgcn_exp2f(x * x * -kLog2e);
-  return 0.5f * poly * t * *e;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.2316419f, __builtin_fabsf(z), 1.0f));
+  // (its coefficients over the root of 2 pi)
+  float poly = __builtin_fmaf(0.530702714f, t, -0.726576014f);
+  poly = __builtin_fmaf(poly, t, 0.710706870f);
+  poly = __builtin_fmaf(poly, t, -0.142248368f);
+  poly = __builtin_fmaf(poly, t, 0.127414796f);
+  *e = __builtin_amdgcn_exp2f(z * (z * (-0.5f * kLog2e)));
+  return poly * t * *e;
 }
 
 // The activation is uniform: one dispatch for a lane's values.  NaN stays NaN.
@@ -115,15 +115,15 @@ __device__ __forceinline__ float linear_act_slope(float z, int act, float slope)
     const float p = logistic_of_exponent(-z * __builtin_fmaf(kGeluB, z * z, kGeluA));
     // z p(u(z)): p + z p (1 - p) u', u' = 2 sqrt(2/pi) (1 + 3 * 0.044715 z^2); beyond |z| = 16, where p is 0 or 1, the
     // cubic term would be infinite times zero
-    const float zc = __builtin_fminf(__builtin_fmaxf(z, -16.0f), 16.0f);
+    const float zc = __builtin_amdgcn_fmed3f(z, -16.0f, 16.0f);
     const float du = __builtin_fmaf(0.21406572f * zc, zc, 1.59576912f);
     return __builtin_fmaf(zc * p * (1.0f - p), du, p);
   }
   case kActGelu: {
     float e;
     const float tail = normal_tail(z, &e);
-    const float zc = __builtin_fminf(__builtin_fmaxf(z, -16.0f), 16.0f);
-    return (z < 0.0f ? tail : 1.0f - tail) + zc * e * 0.39894228040143268f;
+    const float zc = __builtin_amdgcn_fmed3f(z, -16.0f, 16.0f);      // (an infinite one times zero, else)
+    return __builtin_fmaf(zc * 0.39894228040143268f, e, z < 0.0f ? tail : 1.0f - tail);
   }
   default: return 1.0f;
   }

@@ -13,12 +13,13 @@ namespace cummhip {
 #ifdef CUMM_LINEAR_HOST
 
 // Which kernel and how many slices: the least estimated time, in us on 256 CUs.  The figures are fitted (non-negative least
-// squares of the relative error, 12 % on average) to 29 k timings of 2100 random products of all three layouts, bf16: m to
+// squares of the relative error, 12 % on average) to 42 k timings of 2400 random products of all three layouts, bf16: m to
 // 120000, n to 16384, k to 100000.  With them the choice is 4 % slower than the fastest of every kernel and number of
 // slices tried.  R: workgroups per CU, rounded up while there are one or two (one per CU: always), as they are beyond; steps
 // of 64 k.
 //   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
-// 64 x 64 in 2 x 2 x 2 waves and 64 x 128 in 2 x 4, three stages; the others through registers.  Few rows (17 to
+// 64 x 64 in four waves and two stages (rows by the hundred thousand and a step or two: 119985 x 64 x 64 9.5 us against 12.7),
+// or in 2 x 2 x 2 waves and three; 64 x 128 in 2 x 4, three stages; the others through registers.  Few rows (17 to
 // 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
 // (31 x 2376 x 72 4.8 us against 14.1 in eight slices), above them while one round of workgroups does (60 x 5256 x 15680
 // 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 57 us in 64 slices of
@@ -27,12 +28,13 @@ namespace cummhip {
 struct TileFigures {
   double launch, turn, step, operands, partial, join;
 };
-constexpr TileFigures kTiles[5][3] = {
-    {{0, 3.421, 0.221, 0.03681, 0.8072, 2.345}, {0, 2.285, 0.2482, 0, 0.6787, 1.389}, {4.212, 0.7239, 0.277, 0, 0.3323, 1.649}},      // 64 x 64
-    {{3.57, 0, 0.3104, 0.04129, 0.7229, 2.229}, {0, 2.476, 0.3057, 0.05074, 0.6454, 0.411}, {4.838, 1.048, 0.3628, 0.02501, 0.2659, 2.122}},      // 64 x 128
-    {{4.554, 0, 0.418, 0.0259, 0.6964, 1.825}, {0, 3.486, 0.4362, 0.01508, 0.4837, 0}, {6.421, 1.221, 0.5828, 0.02649, 0.2903, 0}},      // 128 x 128
-    {{0, 6.649, 0.6843, 0.03072, 0.5685, 0.8315}, {4.111, 4.333, 0.8235, 0.02194, 0.2804, 0}, {4.111, 4.333, 0.8235, 0.02194, 0.2804, 0}},      // 128 x 256
-    {{8.754, 0, 1.023, 0.04024, 0.4486, 0}, {1.944, 4.234, 1.359, 0.02885, 0.3361, 0}, {1.944, 4.234, 1.359, 0.02885, 0.3361, 0}},      // 256 x 256
+constexpr TileFigures kTiles[6][3] = {
+    {{3.003, 0, 0.2961, 0.1575, 0.6559, 2.241}, {0, 1.805, 0.2707, 0.01193, 0.6338, 1.618}, {3.626, 0.3804, 0.2655, 0.01601, 0.3635, 2.196}},      // 64 x 64, four waves
+    {{0, 3.407, 0.2307, 0.0382, 0.8178, 2.341}, {0, 2.301, 0.2458, 0.00269, 0.6358, 1.569}, {4.167, 0.7239, 0.2754, 0, 0.2664, 2.387}},      // 64 x 64
+    {{3.561, 0, 0.3179, 0.04139, 0.724, 2.238}, {0, 2.456, 0.3213, 0.04474, 0.5992, 0.7795}, {4.777, 1.028, 0.3715, 0.02534, 0.2561, 2.198}},      // 64 x 128
+    {{4.548, 0, 0.4215, 0.03335, 0.6902, 1.861}, {0, 3.524, 0.419, 0.02631, 0.4779, 0}, {5.877, 1.281, 0.5569, 0.03775, 0.3011, 0}},      // 128 x 128
+    {{0, 6.656, 0.6827, 0.03557, 0.576, 0.845}, {3.231, 4.953, 0.794, 0.02276, 0.2717, 0}, {3.231, 4.953, 0.794, 0.02276, 0.2717, 0}},      // 128 x 256
+    {{0, 8.813, 1.027, 0.04948, 0.4428, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}},      // 256 x 256
 };
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
   if (layout == kResult && m <= 16) return {kTileFew, 1};
@@ -42,17 +44,17 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
   if (layout == kResult && m <= 64) {
     const bool two = m <= 32;      // blocks of 16 rows: two workgroups fit a CU, else one
     const double rounds = (double)(((n + 15) / 16 + (two ? 511 : 255)) / (two ? 512 : 256)), steps = (double)((k + 255) / 256);
-    least = two ? 0.8777 + rounds * (2.16 + 0.1743 * steps) : 1.415 + rounds * (2.016 + 0.2803 * steps);
+    least = two ? 1.031 + rounds * (1.989 + 0.1778 * steps) : 1.397 + rounds * (2.037 + 0.2782 * steps);
     best = {kTileFew, 1};
   }
-  constexpr int kShape[5][3] = {{64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
+  constexpr int kShape[6][3] = {{64, 64, kTile64Small}, {64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
   for (int slices = 1; slices <= 256; slices *= 2) {
     if (slices > 1 && k / slices < 128) break;
     const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
-    for (int t = 0; t < 5; ++t) {
+    for (int t = 0; t < 6; ++t) {
       const double wgs = (double)((m + kShape[t][0] - 1) / kShape[t][0]) * (double)((n + kShape[t][1] - 1) / kShape[t][1]) * slices;
       const int regime = wgs <= 256 ? 0 : (wgs <= 512 ? 1 : 2);
-      const double rounds = regime < 2 ? regime + 1.0 : (t >= 3 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
+      const double rounds = regime < 2 ? regime + 1.0 : (t >= 4 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
       const TileFigures &f = kTiles[t][regime];
       const double us = f.launch + rounds * (f.turn + f.step * steps) + f.operands * (operands + (slices == 1 ? sums / 2 : 0.0)) +
                         (slices == 1 ? 0.0 : f.partial * sums * slices + f.join);
@@ -133,6 +135,7 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
       if (p.m <= 64) return few<T, OUT, 4, 4, 2, 3>(p, s);
     }
     return e;
+  case kTile64Small: e = ring<T, OUT, 2, 2, 1, 2, 2, 2, 2, XT, YT>(p, s); break;
   case kTile64: e = ring<T, OUT, 2, 2, 2, 2, 2, 2, 3, XT, YT>(p, s); break;
   case kTile64x128: e = ring<T, OUT, 2, 4, 1, 2, 2, 2, 3, XT, YT>(p, s); break;
   case kTile128:      // (three stages where a CU has one workgroup: 2048^3 21.9 us against 24.9; two of two: 8192 x 1024 x 2048 39 against 48)

@@ -371,7 +371,7 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const NormGrad
 // Gradient through the activation and column sums of it: dz = g act'(z), sums of dz before it is rounded.  A workgroup
 // takes a strip of up to 256 columns (32 pieces) of a block of rows, 256 / pieces rows at a time; its sums go to a row
 // of partial sums, added up in the order of the blocks.
-template <class T>
+template <class T, bool NT>
 __global__ __launch_bounds__(256) void linear_gate_kernel(const LinearGateParams p) {
   __shared__ float lds[256][9];
   const int pieces = 1 << p.shift, lanes = 256 >> p.shift;
@@ -387,8 +387,8 @@ __global__ __launch_bounds__(256) void linear_gate_kernel(const LinearGateParams
       const int64_t at = r + b * lanes;
       g[b].raw = z[b].raw = v4i{0, 0, 0, 0};
       if (at < r1 && count > 0) {
-        g[b].load(p.grad, at * p.ldg + c, count);
-        if (p.pre != nullptr) z[b].load(p.pre, at * p.ldp + c, count);
+        g[b].template load<NT>(p.grad, at * p.ldg + c, count);
+        if (p.pre != nullptr) z[b].template load<NT>(p.pre, at * p.ldp + c, count);
       }
     }
 #pragma unroll
@@ -403,11 +403,9 @@ __global__ __launch_bounds__(256) void linear_gate_kernel(const LinearGateParams
         for (int e = 0; e < 8; ++e) f[e] *= linear_act_slope(zf[e], p.act, p.slope);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += e < count ? f[e] : 0.0f;
+      for (int e = 0; e < 8; ++e) sum[e] += f[e];      // (zeros behind the end: the slope there is finite)
       if (p.dz != nullptr && c < p.ldz) {      // (whole pieces: zeros behind the end of a row)
         Piece<T> out;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = e < count ? f[e] : 0.0f;
         out.round(f);
         out.store(p.dz, at * p.dz_pitch + c, 8);
       }
@@ -434,6 +432,8 @@ __global__ __launch_bounds__(256) void rows_sum_kernel(const float *partial, int
   const int c = blockIdx.x * 16 + threadIdx.x;
   if (threadIdx.x < 16 && c < n) reinterpret_cast<uint16_t *>(dst)[c] = Elem<T>::from_float(total);
 }
+
+constexpr size_t kStreamBytes = (size_t)64 << 20;      // operands that are read past the caches
 
 template <class T, bool NORM, bool CODES, int G, int P, bool LONG = false>
 hipError_t norm_as(const NormParams &p, hipStream_t s) {
@@ -524,8 +524,10 @@ hipError_t launch_linear_gate(LinearGateParams p, int64_t dz_pitch, void *grad_b
   int strips, blocks;
   linear_gate_shape(p.rows, p.n, &p.shift, &strips, &blocks, &p.rows_per_block);
   const dim3 grid((unsigned)strips, (unsigned)blocks);
-  if (bf16) hipLaunchKernelGGL(linear_gate_kernel<BF16>, grid, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL(linear_gate_kernel<F16>, grid, dim3(256), 0, s, p);
+  const bool stream = (size_t)p.rows * (size_t)p.n * 2 >= kStreamBytes;
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, p); };
+  if (bf16) stream ? launch(linear_gate_kernel<BF16, true>) : launch(linear_gate_kernel<BF16, false>);
+  else stream ? launch(linear_gate_kernel<F16, true>) : launch(linear_gate_kernel<F16, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
   if (bf16) hipLaunchKernelGGL(rows_sum_kernel<BF16>, dim3((unsigned)(p.pitch / 16)), dim3(256), 0, s, p.partial, blocks, p.pitch, grad_bias, p.n);

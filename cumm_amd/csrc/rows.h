@@ -18,10 +18,12 @@ typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
 
 template <class T> struct Piece {      // as they lie in memory
   v4i raw;
+  template <bool NT = false>
   __device__ __forceinline__ void load(const void *base, int64_t at, int count) {
     const uint16_t *src = reinterpret_cast<const uint16_t *>(base) + at;
     if (count >= 8) {
-      raw = *reinterpret_cast<const v4i_any *>(src);
+      if constexpr (NT) raw = __builtin_nontemporal_load(reinterpret_cast<const v4i_any *>(src));
+      else raw = *reinterpret_cast<const v4i_any *>(src);
     } else {
       raw = v4i{0, 0, 0, 0};
       uint16_t *h = reinterpret_cast<uint16_t *>(&raw);
