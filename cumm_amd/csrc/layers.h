@@ -17,6 +17,8 @@ struct LinearPlan {
 enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5, kTile64Small = 6 };
 // k in units of two bytes
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k);
+// whether its launch stays below 2^32 threads
+bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n);
 // bytes of the slices' sums (0 = one slice)
 inline int64_t linear_partial_bytes(const LinearPlan &plan, int64_t m, int n) {
   return plan.slices > 1 ? (int64_t)plan.slices * m * ((n + 7) / 8 * 8) * 4 : 0;

@@ -49,7 +49,7 @@ hipError_t fill(const Operand &a, const Operand &b, hipStream_t s) {
   return a.direct() && b.direct() ? hipSuccess : launch_linear_repack(LinearRepack{{a.repack(), b.repack()}}, a.bytes, s);
 }
 
-bool tiles_fit(int64_t m, int64_t n) { return (m + 63) / 64 * ((n + 63) / 64) <= 0x7fffffff; }
+constexpr int kMaxRow = 1 << 30;                     // elements of a row of a norm
 
 const char *linear_checked(const CummHipLinearArgs &a) {
   const bool s8 = a.dtype == CUMM_HIP_S8;
@@ -61,7 +61,6 @@ const char *linear_checked(const CummHipLinearArgs &a) {
     return "linear: rows overlap (a pitch is smaller than its row)";
   if (a.ld_x * size >= kRowBytes || a.ld_weight * size >= kRowBytes || up((int64_t)a.k * size, 128) >= kRowBytes) return "linear: rows of 8 MiB and more are not taken";
   if (s8 && a.k > kMaxWhole) return "linear: sums of more than 131071 products of 8 bits may exceed int32 range";
-  if (!tiles_fit(a.m, a.n)) return "linear: too many outputs for one launch";
   if (a.act_type < 0 || a.act_type > CUMM_HIP_ACT_GELU_TANH) return "linear: unknown activation";
   if (a.m == 0) return nullptr;
   if (!a.x || !a.weight || !a.out) return "linear: x, weight and out must not be null";
@@ -76,6 +75,7 @@ struct LinearCall {
   Operand x, weight;
   LinearPlan plan;
   int64_t k2;      // k in units of two bytes, as the copies have it
+  bool fits;
   void *partial;
   LinearCall(const CummHipLinearArgs &a, Workspace &w) {
     const int size = a.dtype == CUMM_HIP_S8 ? 1 : 2;
@@ -85,9 +85,11 @@ struct LinearCall {
     weight.place(w);
     k2 = up((int64_t)a.k * size, 16) / 2;
     plan = linear_plan(kResult, a.m, a.n, k2);
+    fits = linear_plan_fits(plan, a.m, a.n);
     partial = plan.slices > 1 ? w.take(linear_partial_bytes(plan, a.m, a.n)) : nullptr;
   }
 };
+constexpr char kTooMany[] = "linear: too many outputs for one launch";
 
 hipError_t launch_two_byte(int dtype, LinearLayout layout, const LinearPlan &plan, const LinearParams &p, hipStream_t s) {
   return dtype == CUMM_HIP_BF16 ? launch_linear_bf16(layout, plan, p, s) : launch_linear_f16(layout, plan, p, s);
@@ -102,7 +104,6 @@ const char *linear_grad_checked(const CummHipLinearGradArgs &a) {
   const int64_t most = kRowBytes / 2;
   if (a.ld_grad_out >= most || a.ld_x >= most || a.ld_weight >= most || up(a.n, 64) >= most || up(a.k, 64) >= most)
     return "linear backward: rows of 8 MiB and more are not taken";
-  if (!tiles_fit(a.m, a.k) || !tiles_fit(a.n, a.k)) return "linear backward: too many outputs for one launch";
   if (a.m == 0) return nullptr;
   if (a.grad_x && !a.weight) return "linear backward: the gradient of x needs the weight";
   if (a.grad_weight && !a.x) return "linear backward: the gradient of the weight needs x";
@@ -121,6 +122,7 @@ struct LinearGradCall {
   int64_t ldz;             // elements
   LinearPlan plan_x = {0, 1}, plan_w = {0, 1};
   void *partial_x = nullptr, *partial_w = nullptr;
+  bool fits = true;
   LinearGradCall(const CummHipLinearGradArgs &a, Workspace &w) {
     const bool act = a.act_type != CUMM_HIP_ACT_NONE, products = a.grad_x || a.grad_weight;
     const Operand g = {a.grad_out, a.m, a.n, a.ld_grad_out, 2};
@@ -152,12 +154,14 @@ struct LinearGradCall {
       weight = {a.weight, a.n, a.k, a.ld_weight, 2};
       weight.place(w);
       plan_x = linear_plan(kGradInput, a.m, a.k, a.n);
+      fits = linear_plan_fits(plan_x, a.m, a.k);
       if (plan_x.slices > 1) partial_x = w.take(linear_partial_bytes(plan_x, a.m, a.k));
     }
     if (a.grad_weight) {
       x = {a.x, a.m, a.k, a.ld_x, 2};
       x.place(w);
       plan_w = linear_plan(kGradWeight, a.n, a.k, a.m);
+      fits = fits && linear_plan_fits(plan_w, a.n, a.k);
       if (plan_w.slices > 1) partial_w = w.take(linear_partial_bytes(plan_w, a.n, a.k));
     }
   }
@@ -167,6 +171,7 @@ const char *norm_checked(const CummHipRmsNormArgs &a) {
   const bool norm = a.weight != nullptr;
   if (!two_byte(a.dtype) && !(a.dtype == CUMM_HIP_F32 && !norm && !a.out)) return "rms norm: f16 or bf16 (f32 for rows in 8 bits without a norm)";
   if (a.m < 0 || a.m > kMaxRows || a.k < 1) return "rms norm: rows must not be empty, their number must not exceed int32 range";
+  if (a.k > kMaxRow) return "rms norm: rows of more than 2^30 elements are not taken";
   if (a.ld_x < a.k || (a.residual && a.ld_residual < a.k)) return "rms norm: rows overlap (a pitch is smaller than its row)";
   if (norm && !(a.eps > 0.0f)) return "rms norm: eps must be positive";
   if (!norm && (a.residual || a.total || a.inv_rms)) return "rms norm: no residual, sum or statistics without a norm";
@@ -184,6 +189,7 @@ const char *norm_checked(const CummHipRmsNormArgs &a) {
 const char *norm_grad_checked(const CummHipRmsNormGradArgs &a) {
   if (!two_byte(a.dtype)) return "rms norm backward: f16 or bf16";
   if (a.m < 0 || a.m > kMaxRows || a.k < 1) return "rms norm backward: rows must not be empty, their number must not exceed int32 range";
+  if (a.k > kMaxRow) return "rms norm backward: rows of more than 2^30 elements are not taken";
   if (a.ld_total < a.k || (a.grad_out && a.ld_grad_out < a.k) || (a.grad_total && a.ld_grad_total < a.k))
     return "rms norm backward: rows overlap (a pitch is smaller than its row)";
   if (a.m == 0) return nullptr;
@@ -208,8 +214,8 @@ int64_t cumm_hip_linear_workspace(const CummHipLinearArgs *a) {
   if (!a || linear_checked(*a)) return -1;
   if (a->m == 0) return 0;
   Workspace w = {nullptr};
-  LinearCall call(*a, w);
-  return w.used;
+  const LinearCall call(*a, w);
+  return call.fits ? w.used : -1;
 }
 
 int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
@@ -218,6 +224,7 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
   if (a->m == 0) return CUMM_HIP_OK;
   Workspace w = {reinterpret_cast<char *>(a->workspace)};
   const LinearCall call(*a, w);
+  if (!call.fits) return bad(kTooMany);
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = fill(call.x, call.weight, s);
@@ -251,8 +258,8 @@ int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *a) {
   if (!a || linear_grad_checked(*a)) return -1;
   if (a->m == 0) return 0;
   Workspace w = {nullptr};
-  LinearGradCall call(*a, w);
-  return w.used;
+  const LinearGradCall call(*a, w);
+  return call.fits ? w.used : -1;
 }
 
 int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
@@ -266,6 +273,7 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
   }
   Workspace w = {reinterpret_cast<char *>(a->workspace)};
   const LinearGradCall call(*a, w);
+  if (!call.fits) return bad(kTooMany);
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
   const bool bf16 = a->dtype == CUMM_HIP_BF16;
   hipError_t e = call.gated ? launch_linear_gate(call.gate, call.ldz, a->grad_bias, bf16, s) : hipSuccess;

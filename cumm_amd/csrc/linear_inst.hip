@@ -48,8 +48,9 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
     best = {kTileFew, 1};
   }
   constexpr int kShape[6][3] = {{64, 64, kTile64Small}, {64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
+  const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);      // (more than fill the device many times over need no slices)
   for (int slices = 1; slices <= 256; slices *= 2) {
-    if (slices > 1 && k / slices < 128) break;
+    if (slices > 1 && (k / slices < 128 || tiles * slices > 16384)) break;
     const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
     for (int t = 0; t < 6; ++t) {
       const double wgs = (double)((m + kShape[t][0] - 1) / kShape[t][0]) * (double)((n + kShape[t][1] - 1) / kShape[t][1]) * slices;
@@ -62,6 +63,19 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
     }
   }
   return best;
+}
+
+bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n) {
+  const auto threads = [&](int64_t tm, int64_t tn, int64_t per) { return (m + tm - 1) / tm * ((n + tn - 1) / tn) * per < (int64_t)1 << 32; };
+  switch (plan.tile) {
+  case kTileFew: return threads(m, 16, 512);
+  case kTile64Small: return threads(64, 64, 256);
+  case kTile64: return threads(64, 64, 512);
+  case kTile64x128: return threads(64, 128, 512);
+  case kTile128: return threads(128, 128, 512);
+  case kTile128x256: return threads(128, 256, 512);
+  default: return threads(256, 256, 512);
+  }
 }
 
 hipError_t launch_linear_repack(LinearRepack p, int elem_bytes, hipStream_t s) {

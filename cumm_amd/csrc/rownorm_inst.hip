@@ -112,7 +112,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParam
   __shared__ float2 lds[16];
   constexpr int ROWS = G < 256 ? 256 / G : 1;
   const int lane = threadIdx.x % G;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / G;
   const bool live = row < p.rows;
   const int k = live ? p.k : 0;
   const int trips = LONG ? (p.k + 8 * G * P - 1) / (8 * G * P) : 1;
@@ -439,8 +439,8 @@ template <class T, bool NORM, bool CODES, int G, int P, bool LONG = false>
 hipError_t norm_as(const NormParams &p, hipStream_t s) {
   constexpr int ROWS = G < 256 ? 256 / G : 1;
   const int64_t wgs = (p.rows + ROWS - 1) / ROWS;
-  if (wgs > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((norm_kernel<T, NORM, CODES, G, P, LONG>), dim3((unsigned)wgs), dim3(G < 256 ? 256 : G), 0, s, p);
+  const int64_t wide = std::min<int64_t>(wgs, 1 << 21);      // (a launch has fewer than 2^32 threads along a side)
+  hipLaunchKernelGGL((norm_kernel<T, NORM, CODES, G, P, LONG>), dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(G < 256 ? 256 : G), 0, s, p);
   return hipGetLastError();
 }
 template <class T, bool NORM, bool CODES>

@@ -20,6 +20,7 @@ struct Rows {
     rows = t.numel() / cols;
     pitch = cols;
     if (t.is_contiguous()) return;
+    if (t.dim() != 2) t = t.reshape({-1, cols});      // (a view where the rows are evenly apart)
     if (t.dim() == 2 && (t.stride(1) == 1 || cols == 1) && (rows == 1 || t.stride(0) >= cols)) {
       if (rows > 1) pitch = t.stride(0);
       return;
@@ -56,11 +57,12 @@ std::vector<int64_t> with_last(const Tensor &x, int64_t n) {
 int layer_type(at::ScalarType t) { return t == at::kChar ? CUMM_HIP_S8 : (t == at::kFloat ? CUMM_HIP_F32 : tv_type(t)); }
 
 // out, and what the activation got (undefined unless wanted); scales: of 8-bit operands
-std::pair<Tensor, Tensor> linear_result(const Rows &x, const Rows &w, const Tensor &bias, const Tensor &residual, int64_t act, double slope, at::ScalarType out_type,
+std::pair<Tensor, Tensor> linear_result(const Tensor &x_, const Tensor &w_, const Tensor &bias, const Tensor &residual, int64_t act, double slope, at::ScalarType out_type,
                                         bool want_pre, const Tensor &x_scale, const Tensor &w_scale) {
-  const c10::Device device = x.t.device();
+  const Rows x(x_), w(w_);
+  const c10::Device device = x_.device();
   const auto options = kind_of(out_type, device);
-  const Tensor out = at::empty(with_last(x.t, w.rows), options), pre = want_pre ? at::empty({x.rows, w.rows}, options) : Tensor();
+  const Tensor out = at::empty(with_last(x_, w.rows), options), pre = want_pre ? at::empty({x.rows, w.rows}, options) : Tensor();
   CummHipLinearArgs a = {};
   a.dtype = layer_type(x.t.scalar_type());
   a.out_dtype = layer_type(out_type);
@@ -109,7 +111,7 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
     const Tensor bias = given(bias_), residual = given(residual_);
     // (the sign of a ReLU's result is that of its argument, unless something is added to it)
     const bool by_result = act == CUMM_HIP_ACT_RELU && !residual.defined();
-    const auto got = linear_result(Rows(x), Rows(w), bias, residual, act, slope, x.scalar_type(), act != CUMM_HIP_ACT_NONE && !by_result, Tensor(), Tensor());
+    const auto got = linear_result(x, w, bias, residual, act, slope, x.scalar_type(), act != CUMM_HIP_ACT_NONE && !by_result, Tensor(), Tensor());
     ctx->save_for_backward({save_x ? x : Tensor(), save_w ? w : Tensor(), by_result ? got.first : got.second});
     ctx->saved_data["edges"] = (int64_t)(bias.defined() ? 1 : 0) | (residual.defined() ? 2 : 0);
     ctx->saved_data["act"] = act;
@@ -180,7 +182,7 @@ bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 Tensor linear_of(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &residual, int64_t act, double slope) {
   const c10::Device device = x.device();
   const at::ScalarType type = x.scalar_type();
-  if (!device.is_cuda() || tv_type(type) < 0 || x.dim() < 1 || w.dim() != 2 || !simple(x, device, type) || !simple(w, device, type) || w.size(1) != x.size(-1) ||
+  if (!device.is_cuda() || tv_type(type) < 0 || x.dim() < 1 || w.dim() != 2 || !simple(x, device, type) || !simple(w, device, type) || w.size(1) != x.size(-1) || w.size(0) > INT32_MAX || w.size(1) > INT32_MAX ||
       (bias.defined() && (!simple(bias, device, type) || bias.dim() != 1 || bias.size(0) != w.size(0))) ||
       (residual.defined() && (!simple(residual, device, type) || residual.sizes() != c10::IntArrayRef(with_last(x, w.size(0))))) || traced())
     return Tensor();
@@ -188,14 +190,14 @@ Tensor linear_of(const Tensor &x, const Tensor &w, const Tensor &bias, const Ten
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias) || wants_grad(residual)))
     return LinearLayer::apply(x, w, maybe(bias), maybe(residual), act, slope, wants_grad(w), wants_grad(x));
   at::AutoGradMode no_grad(false);
-  return linear_result(Rows(x), Rows(w), bias, residual, act, slope, type, false, Tensor(), Tensor()).first;
+  return linear_result(x, w, bias, residual, act, slope, type, false, Tensor(), Tensor()).first;
 }
 
 Tensor linear_s8_of(const Tensor &x, const Tensor &x_scale, const Tensor &w, const Tensor &w_scale, const Tensor &bias, const Tensor &residual, int64_t act,
                     double slope, at::ScalarType out_type) {
   const c10::Device device = x.device();
   if (!device.is_cuda() || tv_type(out_type) < 0 || x.dim() < 1 || w.dim() != 2 || !simple(x, device, at::kChar) || !simple(w, device, at::kChar) ||
-      w.size(1) != x.size(-1) || !simple(x_scale, device, at::kFloat) || !simple(w_scale, device, at::kFloat) ||
+      w.size(1) != x.size(-1) || w.size(0) > INT32_MAX || w.size(1) > INT32_MAX || !simple(x_scale, device, at::kFloat) || !simple(w_scale, device, at::kFloat) ||
       x_scale.sizes() != x.sizes().slice(0, x.dim() - 1) || w_scale.dim() != 1 || w_scale.size(0) != w.size(0) ||
       (bias.defined() && (!simple(bias, device, at::kFloat) || bias.dim() != 1 || bias.size(0) != w.size(0))) ||
       (residual.defined() && (!simple(residual, device, out_type) || residual.sizes() != c10::IntArrayRef(with_last(x, w.size(0))))) || traced() ||
@@ -203,7 +205,7 @@ Tensor linear_s8_of(const Tensor &x, const Tensor &x_scale, const Tensor &w, con
     return Tensor();
   const c10::DeviceGuard guard(device);
   at::AutoGradMode no_grad(false);
-  return linear_result(Rows(x), Rows(w), bias, residual, act, slope, out_type, false, x_scale, w_scale).first;
+  return linear_result(x, w, bias, residual, act, slope, out_type, false, x_scale, w_scale).first;
 }
 
 struct NormResult {
@@ -308,7 +310,7 @@ bool norm_fits(const Tensor &x, const Tensor &weight, const Tensor &residual, do
   const c10::Device device = x.device();
   const at::ScalarType type = x.scalar_type();
   return device.is_cuda() && tv_type(type) >= 0 && x.dim() >= 1 && simple(x, device, type) && simple(weight, device, type) && weight.dim() == 1 &&
-         weight.size(0) == x.size(-1) && (!residual.defined() || (simple(residual, device, type) && residual.sizes() == x.sizes())) && eps > 0 && !traced();
+         weight.size(0) == x.size(-1) && x.size(-1) <= INT32_MAX && (!residual.defined() || (simple(residual, device, type) && residual.sizes() == x.sizes())) && eps > 0 && !traced();
 }
 
 // {out}, {out, total}, or nothing where the call is Python's
@@ -325,7 +327,7 @@ std::vector<Tensor> norm_of(const Tensor &x, const Tensor &weight, const Tensor 
 // {codes, scale}, {codes, scale, total}, or nothing; weight undefined: rows in 8 bits without a norm
 std::vector<Tensor> codes_of(const Tensor &x, const Tensor &weight, const Tensor &residual, double eps) {
   if (weight.defined() ? !norm_fits(x, weight, residual, eps)
-                       : !(x.device().is_cuda() && x.dim() >= 1 && (tv_type(x.scalar_type()) >= 0 || x.scalar_type() == at::kFloat) &&
+                       : !(x.device().is_cuda() && x.dim() >= 1 && x.size(-1) <= INT32_MAX && (tv_type(x.scalar_type()) >= 0 || x.scalar_type() == at::kFloat) &&
                            simple(x, x.device(), x.scalar_type()) && !traced()))
     return {};
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual))) return {};

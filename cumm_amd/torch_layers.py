@@ -158,6 +158,7 @@ class _Linear(torch.autograd.Function):
 def _linear_args(name, x, weight, bias, residual, activation, out_dtype, bias_dtype):
     _check(x.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == x.shape[-1] and weight.shape[0] > 0 and weight.shape[1] > 0,
            "%s: x must be [..., K] and weight [N, K]" % name)
+    _check(max(weight.shape) < 1 << 31, "%s: sizes must not exceed int32 range" % name)
     _check(weight.dtype == x.dtype, "%s: x and weight must have the same dtype" % name)
     _on_device(x, weight=weight, bias=bias, residual=residual)
     n = weight.shape[0]
@@ -281,7 +282,7 @@ class _RmsNorm(torch.autograd.Function):
 
 
 def _norm_args(name, x, weight, residual, eps):
-    _check(x.dim() >= 1 and x.shape[-1] > 0, "%s: x must be [..., K]" % name)
+    _check(x.dim() >= 1 and 0 < x.shape[-1] < 1 << 31, "%s: x must be [..., K]" % name)
     _check(x.dtype in _HALVES, "%s: x must be float16 or bfloat16" % name)
     _check(weight.shape == x.shape[-1:] and weight.dtype == x.dtype, "%s: weight must be [%d] of %s" % (name, x.shape[-1], x.dtype))
     _check(eps > 0, "%s: eps must be positive" % name)
@@ -339,7 +340,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         if got is not None:
             return got
     _no_gradient("quantize_rows", x)
-    _check(x.dim() >= 1 and x.shape[-1] > 0, "quantize_rows: x must be [..., K]")
+    _check(x.dim() >= 1 and 0 < x.shape[-1] < 1 << 31, "quantize_rows: x must be [..., K]")
     _check(x.dtype in _HALVES or x.dtype == torch.float32, "quantize_rows: x must be float16, bfloat16 or float32")
     _on_device(x)
     shape = x.shape

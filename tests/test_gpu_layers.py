@@ -104,6 +104,13 @@ def test_linear_pitches_and_alignments(L, m, k, n, pad, lead):
     linear_case(L, torch.float16, m, k, n, "silu", True, True, seed=pad, pad=pad, lead=lead)
 
 
+# every tile in every layout, whole and in slices: large, 128 x 256, 128 x 128 in two and three stages, ends of k inside steps
+@pytest.mark.parametrize("m,k,n", [(4093, 1000, 4088), (4093, 4088, 1000), (1000, 4088, 4093), (66000, 264, 680), (65272, 680, 168), (2040, 2056, 8200),
+                                   (8200, 2040, 1030), (20000, 512, 520), (700, 20000, 500)])
+def test_linear_large_sizes(L, m, k, n):
+    check_gradients(L, "gelu" if k % 16 else "silu", torch.bfloat16 if m % 2 else torch.float16, m, k, n, m % 4 == 0)
+
+
 def test_linear_large_tile(L):
     linear_case(L, torch.bfloat16, 4100, 1000, 4104, "gelu_tanh", True, True)
     linear_case(L, torch.float16, 4100, 520, 4001, "relu", True, False)
@@ -116,6 +123,10 @@ def test_linear_shapes_and_empty(either):
     got = L.linear(x, w, b)
     assert got.shape == (2, 3, 5, 24) and torch.equal(got.view(30, 24), L.linear(x.view(30, 40), w, b))
     assert torch.equal(L.linear(x.transpose(0, 1), w, b), got.transpose(0, 1))
+    wide = normal(g, 2, 3, 5, 64)
+    assert torch.equal(L.linear(wide[..., 8:48], w, b), L.linear(wide[..., 8:48].contiguous(), w, b))
+    assert torch.equal(L.linear(wide[:, :2, 1:, 8:48], w, b), L.linear(wide[:, :2, 1:, 8:48].contiguous(), w, b))
+    assert torch.equal(L.rms_norm(wide[..., 8:48], w[0]), L.rms_norm(wide[..., 8:48].contiguous(), w[0]))
     assert torch.equal(L.linear(x[1, 2, 3], w, b), L.linear(x[1, 2, 3:4], w, b)[0])
     assert L.linear(x[:0], w, b).shape == (0, 3, 5, 24)
     one = normal(g, 1, 1, 1, 24).expand(2, 3, 5, 24)
@@ -152,6 +163,11 @@ def test_linear_out_of_range_numbers_of_activations(L):
 @pytest.mark.parametrize("m,k,n,residual", [(1, 8, 8, True), (3, 33, 17, False), (70, 64, 40, True), (300, 129, 264, False), (2000, 64, 128, True),
                                             (150, 2048, 200, False)])
 def test_linear_gradients(L, act, dtype, m, k, n, residual):
+    check_gradients(L, act, dtype, m, k, n, residual)
+
+
+def check_gradients(L, act, dtype, m, k, n, residual):
+    """The result and all gradients of a call against the formulas."""
     g = gen(m + n)
     x, w, b = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=1 / math.sqrt(k)), normal(g, n, dtype=dtype)
     r = normal(g, m, n, dtype=dtype) if residual else None
@@ -161,7 +177,9 @@ def test_linear_gradients(L, act, dtype, m, k, n, residual):
     got = torch.autograd.grad(out, leaves, dy)
     with torch.no_grad():
         assert torch.equal(out, L.linear(x, w, b, activation=act, residual=r, slope=0.2))
-        z, _ = R.linear(x, w, b, act, r, 0.2)
+        z, want = R.linear(x, w, b, act, r, 0.2)
+        err = 1.13 * (sum_error(x, w, k) + z.abs() * 2.0 ** -23) + z.abs() * 2.0 ** -21 + want.abs() * 2.0 ** -23
+        within(out, want, err * (1 + EPS[dtype]) + half_step(want, dtype), "linear")
         dz = dy.double() * R.slope(z, act, 0.2)
         # the argument is off by the sum's error and its rounding, the slope by at most 1.2 times that (its own
         # slope: 0.8 for the gelus, 0.5 for silu, 0.1 for the logistic function) and 2^-20; a kink may go either way
@@ -231,7 +249,7 @@ def test_linear_gradient_of_strided_and_broadcast_results(either):
         torch.autograd.grad(first.float().sum(), w)
 
 
-S8_SIZES = [(1, 1, 1), (1, 4096, 100), (5, 17, 33), (16, 1024, 256), (40, 80, 24), (64, 4096, 520), (65, 128, 64), (130, 4100, 132), (500, 1003, 777), (2000, 512, 520)]
+S8_SIZES = [(4093, 4096, 4100), (300, 16384, 300), (1100, 8192, 4096), (60000, 64, 70), (1, 1, 1), (1, 4096, 100), (5, 17, 33), (16, 1024, 256), (40, 80, 24), (64, 4096, 520), (65, 128, 64), (130, 4100, 132), (500, 1003, 777), (2000, 512, 520)]
 
 
 @pytest.mark.parametrize("m,k,n", S8_SIZES)

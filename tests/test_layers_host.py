@@ -48,18 +48,19 @@ def refused(fn, args, text):
     (dict(x=AT + 1), "aligned"), (dict(out=AT + 1), "aligned"), (dict(bias=AT + 1), "aligned"), (dict(dtype=S8), "scales"),
     (dict(dtype=S8, x_scale=AT, weight_scale=AT, k=131072, ld_x=131072, ld_weight=131072), "131071"),
     (dict(dtype=S8, x_scale=AT, weight_scale=AT, bias=AT + 2), "aligned"), (dict(m=(1 << 31) - 1, n=1 << 20, ld_out=1 << 20), "too many"),
+    (dict(m=16, n=(1 << 31) - 1, ld_out=(1 << 31) - 1), "too many"),
     (dict(k=127, workspace=AT, workspace_bytes=10), "workspace"), (dict(k=127), "workspace"), (dict(k=127, workspace=AT + 16, workspace_bytes=1 << 30), "256-byte"),
 ])
 def test_linear_refuses(more, text):
     refused(_capi.lib().cumm_hip_linear, linear(**more), text)
-    if text not in ("workspace", "256-byte"):
+    if text not in ("workspace", "256-byte"):      # (what the call refuses has no size of a workspace either)
         assert _capi.lib().cumm_hip_linear_workspace(ctypes.byref(linear(**more))) == -1
 
 
 @pytest.mark.parametrize("more,text", [
     (dict(dtype=S8), "f16 or bf16"), (dict(n=0), "empty"), (dict(act_type=9), "activation"), (dict(ld_grad_out=63), "overlap"), (dict(ld_x=4 << 20), "8 MiB"),
     (dict(weight=None), "needs the weight"), (dict(x=None), "needs x"), (dict(grad_out=None), "null"), (dict(act_type=4), "pre_act"),
-    (dict(grad_out=AT + 1), "aligned"), (dict(), "workspace"),
+    (dict(grad_out=AT + 1), "aligned"), (dict(), "workspace"), (dict(m=(1 << 31) - 1, k=1 << 20, ld_x=1 << 20, ld_weight=1 << 20), "too many"),
 ])
 def test_linear_backward_refuses(more, text):
     refused(_capi.lib().cumm_hip_linear_backward, linear_grad(**more), text)
@@ -67,6 +68,7 @@ def test_linear_backward_refuses(more, text):
 
 @pytest.mark.parametrize("more,text", [
     (dict(dtype=F32), "f16 or bf16"), (dict(dtype=S8), "f16 or bf16"), (dict(k=0), "empty"), (dict(m=-1), "empty"), (dict(ld_x=63), "overlap"),
+    (dict(k=(1 << 30) + 1, ld_x=(1 << 30) + 1), "2.30"),
     (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(residual=AT, ld_residual=64), "sum is written"), (dict(total=AT), "sum is written"),
     (dict(x=None), "null"), (dict(out=None), "null"), (dict(codes=AT, scale=AT), "either"), (dict(out=None, codes=AT), "scale per row"), (dict(scale=AT), "scale per row"),
     (dict(weight=None), "needs its weight"), (dict(weight=None, codes=AT, out=None, scale=AT, inv_rms=AT), "without a norm"), (dict(x=AT + 1), "aligned"),
