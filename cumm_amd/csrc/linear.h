@@ -226,6 +226,9 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const Acc
     }
     return;
   }
+  // (the residual past the L2s, whose lines the other workgroups' steps want, where there are steps: 4096 x 8192 x 2048 131.7 ->
+  // 125.8 us, 8192^3 793 -> 754; 4096 x 4096 x 256 the other way, 23.1 -> 25.6)
+  const bool past = NT && p.k >= 1024;
   Piece<OUT> add[GROUP];
   float row[GROUP];
   const auto fetch = [&](int group) __attribute__((always_inline)) {
@@ -235,7 +238,10 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams &p, const Acc
       const bool in = m < p.m && in_n && group < ALL;
       add[j].raw = v4i{0, 0, 0, 0};
       row[j] = 0.0f;
-      if (p.residual != nullptr && in) add[j].load(p.residual, m * p.ldr + n, count);
+      if (p.residual != nullptr && in) {
+        if (past) add[j].template load<true>(p.residual, m * p.ldr + n, count);
+        else add[j].load(p.residual, m * p.ldr + n, count);
+      }
       if (S8 && in) row[j] = p.y_scale[m];
     }
   };

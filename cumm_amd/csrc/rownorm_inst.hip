@@ -24,12 +24,13 @@ namespace cummhip {
 
 namespace {
 
-// Sum and maximum over the G threads of a row (G = 64, 256 or 1024: waves of a workgroup whose rows are G threads each);
-// what a wave has of both goes through LDS.  All threads of the workgroup come here equally often.
+// Sum and maximum over the G threads of a row: lanes of a wave (G up to 64; narrow rows, as voxels have them, are several
+// to a wave), or whole waves of a workgroup, which exchange what they have through LDS.  All threads of the workgroup
+// come here equally often.
 template <int G>
 __device__ __forceinline__ void row_sum_max(float &sum, float &top, float2 *lds) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
+  for (int off = (G < 64 ? G : 64) / 2; off > 0; off >>= 1) {
     sum += __shfl_xor(sum, off, 64);
     const float other = __shfl_xor(top, off, 64);
     top = other > top || other != other ? other : top;      // (NaN stays)
@@ -105,9 +106,13 @@ __device__ __forceinline__ void write_codes(int8_t *codes, int first, int k, int
   }
 }
 
+// Operands of this size are read, and results written, past the caches: 16384 rows of 4096 with a residual 96 -> 87 us, 8191 of
+// 5120 to 8 bits 58 -> 51, 8192 of 8192 to 8 bits without a norm 38 -> 35.  What is smaller the next launch finds there.
+constexpr size_t kStreamBytes = (size_t)64 << 20;
+
 // G threads per row, P pieces of eight elements each: rows of up to 8 G P elements.  Longer rows (LONG) are read again
 // for the second half, from the cache if it holds them.
-template <class T, bool NORM, bool CODES, int G, int P, bool LONG>
+template <class T, bool NORM, bool CODES, int G, int P, bool LONG, bool NT>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParams p) {
   __shared__ float2 lds[16];
   constexpr int ROWS = G < 256 ? 256 / G : 1;
@@ -125,9 +130,9 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParam
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const int c = first + (lane + j * G) * 8;
-      if (c < k) x[j].load(p.x, row * p.ldx + c, k - c);
+      if (c < k) x[j].template load<NT>(p.x, row * p.ldx + c, k - c);
       if constexpr (NORM) {
-        if (p.residual != nullptr && c < k) r[j].load(p.residual, row * p.ldr + c, k - c);
+        if (p.residual != nullptr && c < k) r[j].template load<NT>(p.residual, row * p.ldr + c, k - c);
       }
     }
 #pragma unroll
@@ -143,7 +148,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParam
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[e] += f[e];
           x[j].round(h);
-          x[j].store(p.total, row * p.k + c, k - c);
+          x[j].template store<NT>(p.total, row * p.k + c, k - c);
           x[j].values(h);
         }
 #pragma unroll
@@ -212,7 +217,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParam
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[e] = h[e] * inv * f[e];
         x[j].round(h);
-        x[j].store(p.out, row * p.k + c, k - c);
+        x[j].template store<NT>(p.out, row * p.k + c, k - c);
       }
     }
   }
@@ -220,96 +225,115 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_kernel(const NormParam
 
 // A workgroup of 1024 threads takes 1024 / G rows at a time, each thread the same columns of all its rows, so that the
 // weight is read once and dw adds up in registers: one row of partial sums per workgroup, added up in order
-// (column_sum.h).  All rows' loads of a trip are on their way before its reduction, the next trip's before its use.
-template <class T, int G, int P>
+// (column_sum.h).  The rows of a trip stay as they lie in memory - their values are worked out twice, before and after the
+// reduction - so that those of the next one can be on their way (AHEAD) in the 128 registers that a thread has: kept as
+// values, 8192 rows of 4096 spill and take 172 us.
+template <class T, int G, int P, bool AHEAD, bool NT>
 __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormGradParams p) {
+  constexpr int ROWS = 1024 / G, WIDTH = 8 * G * P;
+  constexpr int PARTS = ROWS < 16 ? ROWS : 16;      // sums of a column that meet in LDS: of row groups, or of waves
   __shared__ float2 lds[16];
-  __shared__ float sums[G < 1024 ? 8 * G * P : 1];
-  constexpr int ROWS = 1024 / G;
+  __shared__ float sums[PARTS > 1 ? PARTS * WIDTH : 1];
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
   const int k = p.k;
-  float w[P][8], dw[P][8];
+  Piece<T> w[P];
+  float dw[P][8];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     const int c = (lane + j * G) * 8;
-    Piece<T> t;
+    w[j].raw = v4i{0, 0, 0, 0};
+    if (c < k) w[j].load(p.weight, c, k - c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[j][e] = dw[j][e] = 0.0f;
-    if (c < k) {
-      t.load(p.weight, c, k - c);
-      t.values(w[j]);
-    }
+    for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
   }
   const float per = 1.0f / (float)k;
-  Piece<T> h[P], g[P], s[P];
-  float inv = 0.0f;
-  const auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+  struct Row {
+    Piece<T> h[P], g[P], s[P];
+    float inv;
+  };
+  const auto fetch = [&](Row &r, int64_t row) __attribute__((always_inline)) {
     const bool live = row < p.rows;
-    inv = live ? p.inv[row] : 0.0f;
+    r.inv = live ? p.inv[row] : 0.0f;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const int c = (lane + j * G) * 8;
-      h[j].raw = g[j].raw = s[j].raw = v4i{0, 0, 0, 0};
+      r.h[j].raw = r.g[j].raw = r.s[j].raw = v4i{0, 0, 0, 0};
       if (c < k && live) {
-        h[j].load(p.h, row * p.ldh + c, k - c);
-        if (p.grad != nullptr) g[j].load(p.grad, row * p.ldg + c, k - c);
-        if (p.grad_total != nullptr) s[j].load(p.grad_total, row * p.ldt + c, k - c);
+        r.h[j].template load<NT>(p.h, row * p.ldh + c, k - c);
+        if (p.grad != nullptr) r.g[j].template load<NT>(p.grad, row * p.ldg + c, k - c);
+        if (p.grad_total != nullptr) r.s[j].template load<NT>(p.grad_total, row * p.ldt + c, k - c);
       }
     }
   };
   int64_t row = (int64_t)blockIdx.x * ROWS + group;
   const int64_t stride = (int64_t)gridDim.x * ROWS, trips = (p.rows + stride - 1) / stride;
-  fetch(row);
+  Row now, next;
+  fetch(now, row);
   for (int64_t trip = 0; trip < trips; ++trip, row += stride) {
-    float u[P][8], gw[P][8], ds[P][8], dot = 0.0f, none = 0.0f;
-    const float i = inv;
+    if constexpr (AHEAD) fetch(next, row + stride);
+    float dot = 0.0f, none = 0.0f;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      h[j].values(u[j]);
-      g[j].values(gw[j]);
-      s[j].values(ds[j]);
+      float u[8], g[8], f[8];
+      now.h[j].values(u);
+      now.g[j].values(g);
+      w[j].values(f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        u[j][e] *= i;
-        dw[j][e] = __builtin_fmaf(gw[j][e], u[j][e], dw[j][e]);
-        gw[j][e] *= w[j][e];
-        dot = __builtin_fmaf(gw[j][e], u[j][e], dot);
+        u[e] *= now.inv;
+        dw[j][e] = __builtin_fmaf(g[e], u[e], dw[j][e]);
+        dot = __builtin_fmaf(g[e] * f[e], u[e], dot);
       }
     }
-    const bool live = row < p.rows;
-    fetch(row + stride);
     row_sum_max<G>(dot, none, lds);
     const float mean = dot * per;
-    if (!live || p.grad_in == nullptr) continue;
+    if (row < p.rows && p.grad_in != nullptr) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const int c = (lane + j * G) * 8;
-      if (c >= k) continue;
-      float d[8];
+      for (int j = 0; j < P; ++j) {
+        const int c = (lane + j * G) * 8;
+        if (c >= k) continue;
+        float u[8], g[8], f[8], d[8];
+        now.h[j].values(u);
+        now.g[j].values(g);
+        now.s[j].values(d);
+        w[j].values(f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = __builtin_fmaf(i, gw[j][e] - u[j][e] * mean, ds[j][e]);
-      Piece<T> out;
-      out.round(d);
-      out.store(p.grad_in, row * (int64_t)k + c, k - c);
+        for (int e = 0; e < 8; ++e) d[e] = __builtin_fmaf(now.inv, g[e] * f[e] - u[e] * now.inv * mean, d[e]);
+        Piece<T> out;
+        out.round(d);
+        out.template store<NT>(p.grad_in, row * (int64_t)k + c, k - c);
+      }
     }
+    if constexpr (AHEAD) now = next;
+    else fetch(now, row + stride);
   }
   if (p.partial == nullptr) return;
-  if constexpr (ROWS > 1) {      // the row groups' sums, in their order
-    for (int r = 0; r < ROWS; ++r) {
-      if (group == r) {
+  float *to = p.partial + (int64_t)blockIdx.x * p.pitch;
+  if constexpr (PARTS > 1) {
+    // the rows that share a wave, then the waves' or groups' sums in their order
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-          float *at = sums + (lane + j * G) * 8;
+    for (int off = 32; off >= G; off >>= 1)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) at[e] = r == 0 ? dw[j][e] : at[e] + dw[j][e];
-        }
-      }
-      __syncthreads();
+      for (int j = 0; j < P; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[j][e] += __shfl_xor(dw[j][e], off, 64);
+    const int part = G < 64 ? threadIdx.x >> 6 : group;
+    if (G >= 64 || (threadIdx.x & 63) < G) {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[part * WIDTH + (lane + j * G) * 8 + e] = dw[j][e];
     }
-    float *to = p.partial + (int64_t)blockIdx.x * p.pitch;
-    for (int c = threadIdx.x; c < p.pitch; c += 1024) to[c] = c < 8 * G * P ? sums[c] : 0.0f;
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.pitch; c += 1024) {
+      float t = 0.0f;
+      if (c < WIDTH) {
+#pragma unroll
+        for (int r = 0; r < PARTS; ++r) t += sums[r * WIDTH + c];
+      }
+      to[c] = t;
+    }
   } else {
-    float *to = p.partial + (int64_t)blockIdx.x * p.pitch;
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       const int c = (lane + j * G) * 8;
@@ -320,15 +344,22 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormGradParam
   }
 }
 
-// Rows longer than the registers of a workgroup hold: one row per workgroup and trip, read twice.  dw of a
-// workgroup adds up in its row of the partial sums.
-template <class T>
+// Rows longer than the registers of a workgroup hold: one row per workgroup and trip, read twice.  dw of a workgroup adds
+// up in LDS, [element of a piece][piece], or, of the longest rows, in its row of the partial sums.
+constexpr int kLongInLds = 32768;
+template <class T, bool IN_LDS>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const NormGradParams p) {
   __shared__ float2 lds[16];
+  __shared__ float sums[IN_LDS ? kLongInLds : 1];
   const int k = p.k, lane = threadIdx.x;
   float *mine = p.partial != nullptr ? p.partial + (int64_t)blockIdx.x * p.pitch : nullptr;
+  const auto at = [&](int c, int e) -> float & { return IN_LDS ? sums[e * (kLongInLds / 8) + (c >> 3)] : mine[c + e]; };
+  if (mine != nullptr) {
+    for (int c = lane * 8; c < p.pitch; c += 8192)      // (each thread its own columns throughout)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) at(c, e) = 0.0f;
+  }
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const bool first_row = row == blockIdx.x;
     const float i = p.inv[row];
     float dot = 0.0f, none = 0.0f, mean = 0.0f;
     for (int pass = 0; pass < 2; ++pass) {
@@ -339,19 +370,19 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const NormGrad
         w.load(p.weight, c, k - c);
         g.raw = s.raw = v4i{0, 0, 0, 0};
         if (p.grad != nullptr) g.load(p.grad, row * p.ldg + c, k - c);
+        if (pass == 1 && p.grad_total != nullptr) s.load(p.grad_total, row * p.ldt + c, k - c);
         h.values(u);
         g.values(gv);
         w.values(wv);
+        s.values(sv);
         if (pass == 0) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             u[e] *= i;
             dot = __builtin_fmaf(gv[e] * wv[e], u[e], dot);
-            if (mine != nullptr) mine[c + e] = __builtin_fmaf(gv[e], u[e], first_row ? 0.0f : mine[c + e]);
+            if (mine != nullptr) at(c, e) = __builtin_fmaf(gv[e], u[e], at(c, e));
           }
         } else if (p.grad_in != nullptr) {
-          if (p.grad_total != nullptr) s.load(p.grad_total, row * p.ldt + c, k - c);
-          s.values(sv);
           float d[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) d[e] = __builtin_fmaf(i, gv[e] * wv[e] - u[e] * i * mean, sv[e]);
@@ -365,6 +396,11 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(const NormGrad
         mean = dot / (float)k;
       }
     }
+  }
+  if (IN_LDS && mine != nullptr) {
+    for (int c = lane * 8; c < p.pitch; c += 8192)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mine[c + e] = at(c, e);
   }
 }
 
@@ -433,25 +469,33 @@ __global__ __launch_bounds__(256) void rows_sum_kernel(const float *partial, int
   if (threadIdx.x < 16 && c < n) reinterpret_cast<uint16_t *>(dst)[c] = Elem<T>::from_float(total);
 }
 
-constexpr size_t kStreamBytes = (size_t)64 << 20;      // operands that are read past the caches
-
 template <class T, bool NORM, bool CODES, int G, int P, bool LONG = false>
 hipError_t norm_as(const NormParams &p, hipStream_t s) {
   constexpr int ROWS = G < 256 ? 256 / G : 1;
   const int64_t wgs = (p.rows + ROWS - 1) / ROWS;
   const int64_t wide = std::min<int64_t>(wgs, 1 << 21);      // (a launch has fewer than 2^32 threads along a side)
-  hipLaunchKernelGGL((norm_kernel<T, NORM, CODES, G, P, LONG>), dim3((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), dim3(G < 256 ? 256 : G), 0, s, p);
+  const dim3 grid((unsigned)wide, (unsigned)((wgs + wide - 1) / wide)), block(G < 256 ? 256 : G);
+  if (!LONG && (size_t)p.rows * (size_t)p.k * Elem<T>::kBytes >= kStreamBytes) hipLaunchKernelGGL((norm_kernel<T, NORM, CODES, G, P, LONG, !LONG>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((norm_kernel<T, NORM, CODES, G, P, LONG, false>), grid, block, 0, s, p);
   return hipGetLastError();
 }
+// Two pieces a thread throughout, for the loads that it has on their way (20000 rows of 1500 with a residual 54 us with one piece
+// and 256 threads, 45 with two and 128), as many threads as that takes; four where a row is quantised alone, which is half
+// the loads (8192 rows of 8192 40 us with two, 36 with four), and in rows above 8192, where whole workgroups wait for
+// each other at the reduction (4000 of 16384 to 8 bits 46 us with 1024 threads, 37 with 512).  Rows of up to 512 share waves
+// (30000 of 64 12.6 us with a wave each, 6.4 with eight threads).
 template <class T, bool NORM, bool CODES>
 hipError_t norm_of(const NormParams &p, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
-  if (p.k <= 512) return norm_as<T, NORM, CODES, 64, 1>(p, s);
+  if (p.k <= 64) return norm_as<T, NORM, CODES, 8, 1>(p, s);
+  if (p.k <= 128) return norm_as<T, NORM, CODES, 8, 2>(p, s);
+  if (p.k <= 256) return norm_as<T, NORM, CODES, 16, 2>(p, s);
+  if (p.k <= 512) return norm_as<T, NORM, CODES, 32, 2>(p, s);
   if (p.k <= 1024) return norm_as<T, NORM, CODES, 64, 2>(p, s);
-  if (p.k <= 2048) return norm_as<T, NORM, CODES, 256, 1>(p, s);
+  if (p.k <= 2048) return norm_as<T, NORM, CODES, 128, 2>(p, s);
   if (p.k <= 4096) return norm_as<T, NORM, CODES, 256, 2>(p, s);
-  if (p.k <= 8192) return norm_as<T, NORM, CODES, 256, 4>(p, s);
-  if (p.k <= 16384) return norm_as<T, NORM, CODES, 1024, 2>(p, s);
+  if (p.k <= 8192) return NORM ? norm_as<T, NORM, CODES, 512, 2>(p, s) : norm_as<T, NORM, CODES, 256, 4>(p, s);
+  if (p.k <= 16384) return norm_as<T, NORM, CODES, 512, 4>(p, s);
   if (p.k <= 32768) return norm_as<T, NORM, CODES, 1024, 4>(p, s);
   return norm_as<T, NORM, CODES, 1024, 4, true>(p, s);
 }
@@ -459,13 +503,24 @@ hipError_t norm_of(const NormParams &p, hipStream_t s) {
 template <class T>
 hipError_t norm_backward_of(const NormGradParams &p, hipStream_t s) {
   const dim3 grid((unsigned)p.blocks);
-  if (p.k <= 512) hipLaunchKernelGGL((norm_backward_kernel<T, 64, 1>), grid, dim3(1024), 0, s, p);
-  else if (p.k <= 1024) hipLaunchKernelGGL((norm_backward_kernel<T, 64, 2>), grid, dim3(1024), 0, s, p);
-  else if (p.k <= 2048) hipLaunchKernelGGL((norm_backward_kernel<T, 256, 1>), grid, dim3(1024), 0, s, p);
-  else if (p.k <= 4096) hipLaunchKernelGGL((norm_backward_kernel<T, 256, 2>), grid, dim3(1024), 0, s, p);
-  else if (p.k <= 8192) hipLaunchKernelGGL((norm_backward_kernel<T, 1024, 1>), grid, dim3(1024), 0, s, p);
-  else if (p.k <= 16384) hipLaunchKernelGGL((norm_backward_kernel<T, 1024, 2>), grid, dim3(1024), 0, s, p);
-  else hipLaunchKernelGGL(norm_backward_long_kernel<T>, grid, dim3(1024), 0, s, p);
+  const bool stream = (size_t)p.rows * (size_t)p.k * 2 >= kStreamBytes;
+  const auto launch = [&](auto past, auto kept) {
+    if (stream) hipLaunchKernelGGL(past, grid, dim3(1024), 0, s, p);
+    else hipLaunchKernelGGL(kept, grid, dim3(1024), 0, s, p);
+  };
+#define CUMM_NORM(G, P, AHEAD) launch(norm_backward_kernel<T, G, P, AHEAD, true>, norm_backward_kernel<T, G, P, AHEAD, false>)
+  if (p.k <= 64) CUMM_NORM(8, 1, true);
+  else if (p.k <= 128) CUMM_NORM(16, 1, true);
+  else if (p.k <= 256) CUMM_NORM(32, 1, true);
+  else if (p.k <= 512) CUMM_NORM(64, 1, true);
+  else if (p.k <= 1024) CUMM_NORM(128, 1, true);
+  else if (p.k <= 2048) CUMM_NORM(256, 1, true);
+  else if (p.k <= 4096) CUMM_NORM(512, 1, true);
+  else if (p.k <= 8192) CUMM_NORM(1024, 1, true);
+  else if (p.k <= 16384) CUMM_NORM(1024, 2, false);      // (two rows of them do not fit the registers)
+#undef CUMM_NORM
+  else if (p.k <= kLongInLds) hipLaunchKernelGGL((norm_backward_long_kernel<T, true>), grid, dim3(1024), 0, s, p);
+  else hipLaunchKernelGGL((norm_backward_long_kernel<T, false>), grid, dim3(1024), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
   hipLaunchKernelGGL(rows_sum_kernel<T>, dim3((unsigned)(p.pitch / 16)), dim3(256), 0, s, p.partial, p.blocks, p.pitch, p.grad_weight, p.k);
@@ -492,11 +547,14 @@ hipError_t launch_norm(const NormParams &p, int dtype, hipStream_t s) {
   return norm ? (codes ? norm_of<BF16, true, true>(p, s) : norm_of<BF16, true, false>(p, s)) : norm_of<BF16, false, true>(p, s);
 }
 
-// Workgroups of the backward pass: two rounds of the device's 2 x 256 resident ones at most, a row group each at least
+// Workgroups of the backward pass: one per CU, which is what its registers allow (8192 rows of 4096 52 us, with two 57), a row
+// group each at least
+constexpr int kNormBlocks = 256;
 int norm_backward_blocks(int64_t rows, int k) {
-  const int at_once = k <= 1024 ? 16 : (k <= 4096 ? 4 : 1);
+  int at_once = 128;      // rows: 1024 threads of eight columns each
+  while (at_once > 1 && k > 8192 / at_once) at_once /= 2;
   const int64_t wgs = (rows + at_once - 1) / at_once;
-  return (int)(wgs < 512 ? (wgs > 0 ? wgs : 1) : 512);
+  return (int)(wgs < kNormBlocks ? (wgs > 0 ? wgs : 1) : kNormBlocks);
 }
 hipError_t launch_norm_backward(const NormGradParams &p, bool bf16, hipStream_t s) {
   return bf16 ? norm_backward_of<BF16>(p, s) : norm_backward_of<F16>(p, s);

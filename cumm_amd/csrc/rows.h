@@ -53,11 +53,17 @@ template <class T> struct Piece {      // as they lie in memory
 };
 template <> struct Piece<F32> {
   v4i raw[2];
+  template <bool NT = false>
   __device__ __forceinline__ void load(const void *base, int64_t at, int count) {
     const int *src = reinterpret_cast<const int *>(base) + at;
     if (count >= 8) {
-      raw[0] = *reinterpret_cast<const v4i_any4 *>(src);
-      raw[1] = *reinterpret_cast<const v4i_any4 *>(src + 4);
+      if constexpr (NT) {
+        raw[0] = __builtin_nontemporal_load(reinterpret_cast<const v4i_any4 *>(src));
+        raw[1] = __builtin_nontemporal_load(reinterpret_cast<const v4i_any4 *>(src + 4));
+      } else {
+        raw[0] = *reinterpret_cast<const v4i_any4 *>(src);
+        raw[1] = *reinterpret_cast<const v4i_any4 *>(src + 4);
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) raw[e >> 2][e & 3] = e < count ? src[e] : 0;
