@@ -41,6 +41,7 @@ def _units():
              ("order", os.path.join(CSRC, "order_inst.hip"), []),
              ("layers_api", os.path.join(CSRC, "layers_api.hip"), []),
              ("rownorm", os.path.join(CSRC, "rownorm_inst.hip"), []),
+             ("linear_narrow", os.path.join(CSRC, "linear_narrow_inst.hip"), []),
              ("linear_host", os.path.join(CSRC, "linear_inst.hip"), ["-DCUMM_LINEAR_HOST"]),
              ("linear_s8", os.path.join(CSRC, "linear_inst.hip"), ["-DCUMM_LINEAR_S8"])]
     for tag, name in ELEMS:

@@ -42,6 +42,18 @@ struct LinearGateParams {
 };
 void linear_gate_shape(int64_t rows, int n, int *shift, int *strips, int *blocks, int64_t *per);
 hipError_t launch_linear_gate(LinearGateParams p, int64_t dz_pitch, void *grad_bias, bool bf16, hipStream_t s);
+// The whole backward pass of n and k up to kLinearNarrow, multiples of 8 (linear_narrow_inst.hip)
+constexpr int kLinearNarrow = 128;
+struct LinearNarrowParams {
+  const void *x, *grad, *weight, *bias;      // [rows, k], [rows, n], [n, k], [n] or NULL; x and weight NULL where nothing wants them
+  void *grad_x, *grad_weight, *grad_bias;    // dense; each may be NULL
+  float *partial;                            // linear_narrow_bytes
+  int64_t rows, ldx, ldg, ldw;               // elements
+  int32_t n, k, act;
+  float slope;
+};
+int64_t linear_narrow_bytes(int64_t rows, int n, int k);
+hipError_t launch_linear_narrow_backward(const LinearNarrowParams &p, bool bf16, hipStream_t s);
 // two-byte elements (a kernel: memset nodes of captured graphs have given wrong results on replays)
 hipError_t launch_rows_zero(void *dst, int64_t elements, hipStream_t s);
 

@@ -108,8 +108,11 @@ const char *linear_grad_checked(const CummHipLinearGradArgs &a) {
   if (a.grad_x && !a.weight) return "linear backward: the gradient of x needs the weight";
   if (a.grad_weight && !a.x) return "linear backward: the gradient of the weight needs x";
   if (!a.grad_out) return "linear backward: grad_out must not be null";
-  if (a.act_type != CUMM_HIP_ACT_NONE && !a.pre_act) return "linear backward: the activation's argument (pre_act) is missing";
-  for (const void *p : {a.grad_out, a.pre_act, a.x, a.weight, (const void *)a.grad_x, (const void *)a.grad_weight, (const void *)a.grad_bias})
+  if (a.from_inputs) {
+    if (a.n % 8 || a.k % 8 || a.n > kLinearNarrow || a.k > kLinearNarrow) return "linear backward: from the inputs only where n and k are multiples of 8, up to 128";
+    if (a.act_type != CUMM_HIP_ACT_NONE && (!a.x || !a.weight)) return "linear backward: from the inputs, x and weight must not be null";
+  } else if (a.act_type != CUMM_HIP_ACT_NONE && !a.pre_act) return "linear backward: the activation's argument (pre_act) is missing";
+  for (const void *p : {a.grad_out, a.pre_act, a.x, a.weight, a.bias, (const void *)a.grad_x, (const void *)a.grad_weight, (const void *)a.grad_bias})
     if (!on(p, 2)) return "linear backward: a pointer is not aligned to its elements";
   return nullptr;
 }
@@ -257,6 +260,7 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
 int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *a) {
   if (!a || linear_grad_checked(*a)) return -1;
   if (a->m == 0) return 0;
+  if (a->from_inputs) return up(linear_narrow_bytes(a->m, a->n, a->k), 256);
   Workspace w = {nullptr};
   const LinearGradCall call(*a, w);
   return call.fits ? w.used : -1;
@@ -270,6 +274,13 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
     hipError_t e = a->grad_weight ? launch_rows_zero(a->grad_weight, (int64_t)a->n * a->k, s) : hipSuccess;
     if (e == hipSuccess && a->grad_bias) e = launch_rows_zero(a->grad_bias, a->n, s);
     return launched(e);
+  }
+  if (a->from_inputs) {
+    if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, cumm_hip_linear_backward_workspace(a))) return bad(e);
+    if (!a->grad_x && !a->grad_weight && !a->grad_bias) return CUMM_HIP_OK;
+    const LinearNarrowParams p = {a->x, a->grad_out, a->weight, a->bias, a->grad_x, a->grad_weight, a->grad_bias, reinterpret_cast<float *>(a->workspace),
+                                  a->m, a->ld_x, a->ld_grad_out, a->ld_weight, a->n, a->k, a->act_type, a->act_alpha};
+    return launched(launch_linear_narrow_backward(p, a->dtype == CUMM_HIP_BF16, s));
   }
   Workspace w = {reinterpret_cast<char *>(a->workspace)};
   const LinearGradCall call(*a, w);

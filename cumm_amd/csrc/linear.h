@@ -129,6 +129,23 @@ __device__ __forceinline__ float linear_act_slope(float z, int act, float slope)
   }
 }
 
+// Eight of them, multiplied into g: one branch for all
+__device__ __forceinline__ void linear_act_slopes(float (&g)[8], const v4f &lo, const v4f &hi, int act, float slope) {
+  const auto all = [&](auto one) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] *= linear_act_slope(e < 4 ? lo[e] : hi[e - 4], decltype(one)::value, slope);
+  };
+  switch (act) {
+  case kActRelu: all(std::integral_constant<int, kActRelu>{}); break;
+  case kActLeakyRelu: all(std::integral_constant<int, kActLeakyRelu>{}); break;
+  case kActSigmoid: all(std::integral_constant<int, kActSigmoid>{}); break;
+  case kActSilu: all(std::integral_constant<int, kActSilu>{}); break;
+  case kActGelu: all(std::integral_constant<int, kActGelu>{}); break;
+  case kActGeluTanh: all(std::integral_constant<int, kActGeluTanh>{}); break;
+  default: break;
+  }
+}
+
 // Bias of columns n .. n + 7, and what the accumulators are multiplied by (8-bit operands)
 template <class OUT, bool S8>
 __device__ __forceinline__ void linear_columns(const LinearParams &p, int n, float (&bias)[8], float (&scale)[8]) {

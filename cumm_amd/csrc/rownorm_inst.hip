@@ -435,8 +435,7 @@ __global__ __launch_bounds__(256) void linear_gate_kernel(const LinearGateParams
       g[b].values(f);
       z[b].values(zf);
       if (p.pre != nullptr) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= linear_act_slope(zf[e], p.act, p.slope);
+        linear_act_slopes(f, v4f{zf[0], zf[1], zf[2], zf[3]}, v4f{zf[4], zf[5], zf[6], zf[7]}, p.act, p.slope);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] += f[e];      // (zeros behind the end: the slope there is finite)

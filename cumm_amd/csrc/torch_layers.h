@@ -109,10 +109,15 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_,
                         const std::optional<Tensor> &residual_, int64_t act, double slope, bool save_x, bool save_w) {
     const Tensor bias = given(bias_), residual = given(residual_);
-    // (the sign of a ReLU's result is that of its argument, unless something is added to it)
-    const bool by_result = act == CUMM_HIP_ACT_RELU && !residual.defined();
-    const auto got = linear_result(x, w, bias, residual, act, slope, x.scalar_type(), act != CUMM_HIP_ACT_NONE && !by_result, Tensor(), Tensor());
-    ctx->save_for_backward({save_x ? x : Tensor(), save_w ? w : Tensor(), by_result ? got.first : got.second});
+    // what the activation got: of few channels worked out again in the backward pass; the sign of a ReLU's result is that of
+    // its argument, unless something is added to it
+    const auto narrow = [](int64_t c) { return c % 8 == 0 && c <= CUMM_HIP_LINEAR_NARROW; };
+    const bool again = narrow(w.size(0)) && narrow(w.size(1)), whole = again && act != CUMM_HIP_ACT_NONE;
+    const bool by_result = act == CUMM_HIP_ACT_RELU && !residual.defined() && !again;
+    const bool keep = act != CUMM_HIP_ACT_NONE && !by_result && !again;
+    const auto got = linear_result(x, w, bias, residual, act, slope, x.scalar_type(), keep, Tensor(), Tensor());
+    ctx->save_for_backward({save_x || whole ? x : Tensor(), save_w || whole ? w : Tensor(), whole ? bias : (by_result ? got.first : got.second)});
+    ctx->saved_data["again"] = again;
     ctx->saved_data["edges"] = (int64_t)(bias.defined() ? 1 : 0) | (residual.defined() ? 2 : 0);
     ctx->saved_data["act"] = act;
     ctx->saved_data["slope"] = slope;
@@ -139,29 +144,37 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
       a.dtype = layer_type(grad.scalar_type());
       a.m = g.rows;
       a.n = (int32_t)g.cols;
-      a.k = 1;
+      a.k = 8;
       a.grad_out = g.at();
       a.ld_grad_out = g.pitch;
-      if (saved[2].defined()) {
+      Tensor bias;
+      a.from_inputs = ctx->saved_data["again"].toBool();
+      if (saved[2].defined() && a.from_inputs) {
+        a.bias = (bias = saved[2].contiguous()).data_ptr();
+      } else if (saved[2].defined()) {
         a.pre_act = saved[2].data_ptr();
         a.ld_pre_act = g.cols;
       }
       a.act_type = (int32_t)ctx->saved_data["act"].toInt();
       a.act_alpha = (float)ctx->saved_data["slope"].toDouble();
-      if (need[0]) {
+      if (saved[1].defined()) {
         w = Rows(saved[1]);
         a.k = (int32_t)w.cols;
-        result[0] = at::empty(ctx->saved_data["shape"].toIntVector(), options);
         a.weight = w.at();
         a.ld_weight = w.pitch;
+      }
+      if (saved[0].defined()) {
+        x = Rows(saved[0]);
+        a.k = (int32_t)x.cols;
+        a.x = x.at();
+        a.ld_x = x.pitch;
+      }
+      if (need[0]) {
+        result[0] = at::empty(ctx->saved_data["shape"].toIntVector(), options);
         a.grad_x = result[0].data_ptr();
       }
       if (need[1]) {
-        x = Rows(saved[0]);
-        a.k = (int32_t)x.cols;
-        result[1] = at::empty({g.cols, x.cols}, options);
-        a.x = x.at();
-        a.ld_x = x.pitch;
+        result[1] = at::empty({g.cols, (int64_t)a.k}, options);
         a.grad_weight = result[1].data_ptr();
       }
       if (need[2]) {

@@ -118,12 +118,15 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act: int, slope: float):
-        # (the sign of a ReLU's result is that of its argument, unless something is added to it)
-        by_result = act == ACTIVATIONS["relu"] and residual is None
-        out, pre = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, act != 0 and not by_result)
+        # what the activation got: of few channels worked out again in the backward pass; the sign of a ReLU's result is that of
+        # its argument, unless something is added to it
+        ctx.again = all(c % 8 == 0 and c <= _capi.LINEAR_NARROW for c in weight.shape)
+        whole = ctx.again and act != 0
+        by_result = act == ACTIVATIONS["relu"] and residual is None and not ctx.again
+        out, pre = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, act != 0 and not by_result and not ctx.again)
         ctx.act, ctx.slope, ctx.n = act, slope, weight.shape[0]
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight if ctx.needs_input_grad[0] else None,
-                              out if by_result else pre)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] or whole else None, weight if ctx.needs_input_grad[0] or whole else None,
+                              bias if whole else (out if by_result else pre))
         return out
 
     @staticmethod
@@ -135,19 +138,26 @@ class _Linear(torch.autograd.Function):
         if need_x or need_w or need_b:
             lib, g = _capi.lib(), _rows(grad)
             m, n = g.shape
-            k = (x if x is not None else weight).shape[1] if need_x or need_w else 1
+            k = next((t.shape[1] for t in (x, weight) if t is not None), 8)
             with _Device(g.device):
                 a = _capi.LinearGradArgs()
                 a.dtype, a.m, a.n, a.k, a.grad_out, a.ld_grad_out = _TYPES[g.dtype], m, n, k, g.data_ptr(), _pitch(g)
-                if pre is not None:
+                a.from_inputs = ctx.again
+                if pre is not None and ctx.again:
+                    a.bias = pre.data_ptr()
+                elif pre is not None:
                     a.pre_act, a.ld_pre_act = pre.data_ptr(), n
                 a.act_type, a.act_alpha = ctx.act, ctx.slope
+                if x is not None:
+                    a.x, a.ld_x = x.data_ptr(), _pitch(x)
+                if weight is not None:
+                    a.weight, a.ld_weight = weight.data_ptr(), _pitch(weight)
                 if need_x:
                     grad_x = torch.empty((m, k), dtype=g.dtype, device=g.device)
-                    a.weight, a.ld_weight, a.grad_x = weight.data_ptr(), _pitch(weight), grad_x.data_ptr()
+                    a.grad_x = grad_x.data_ptr()
                 if need_w:
                     grad_w = torch.empty((n, k), dtype=g.dtype, device=g.device)
-                    a.x, a.ld_x, a.grad_weight = x.data_ptr(), _pitch(x), grad_w.data_ptr()
+                    a.grad_weight = grad_w.data_ptr()
                 if need_b:
                     grad_b = torch.empty(n, dtype=g.dtype, device=g.device)
                     a.grad_bias = grad_b.data_ptr()
@@ -177,7 +187,8 @@ def _linear_args(name, x, weight, bias, residual, activation, out_dtype, bias_dt
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "none",
            residual: Optional[torch.Tensor] = None, slope: float = 0.01) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual`` for x [..., K], weight [N, K] (f16 / bf16); one rounding.  Differentiable in
-    all four tensors (once).  ``slope`` is that of "leaky_relu"."""
+    all four tensors (once); with N and K multiples of 8 up to 128, the backward pass works out what the activation got from x,
+    weight and bias, which are kept for that.  ``slope`` is that of "leaky_relu"."""
     native = _native()
     if native is not None and activation in ACTIVATIONS:
         out = native.layer_linear(x, weight, bias, residual, ACTIVATIONS[activation], slope)

@@ -540,7 +540,10 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
  * cumm_hip_linear_backward: the gradients for grad_out [m, n], each NULL where it is not wanted:
  *     dz = grad_out act'(pre_act);  grad_x = dz weight [m, k];  grad_weight = dz^T x [n, k];  grad_bias = sum of dz's rows
  *   (the residual's is grad_out).  dz is rounded to dtype for the two products, not for the sum.  pre_act NULL: only with
- *   CUMM_HIP_ACT_NONE; for CUMM_HIP_ACT_RELU without a residual, out serves as well.  m == 0 gives zeros. */
+ *   CUMM_HIP_ACT_NONE; for CUMM_HIP_ACT_RELU without a residual, out serves as well.  m == 0 gives zeros.
+ *   from_inputs != 0, for n and k that are multiples of 8 up to CUMM_HIP_LINEAR_NARROW: one pass over the rows that works
+ *   out what the activation got from x, weight and bias ([n] or NULL; an activation needs the first two); pre_act is not read. */
+#define CUMM_HIP_LINEAR_NARROW 128
 #define CUMM_HIP_ACT_SILU 4
 #define CUMM_HIP_ACT_GELU 5        /* x Phi(x), by erf */
 #define CUMM_HIP_ACT_GELU_TANH 6
@@ -568,6 +571,8 @@ typedef struct CummHipLinearGradArgs {
   void *grad_x, *grad_weight, *grad_bias;        /* dense */
   int32_t act_type;
   float act_alpha;
+  int32_t from_inputs;
+  const void *bias;
   void *workspace;
   size_t workspace_bytes;
 } CummHipLinearGradArgs;

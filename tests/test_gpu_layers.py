@@ -200,6 +200,126 @@ def check_gradients(L, act, dtype, m, k, n, residual):
             assert torch.equal(got[3], dy)
 
 
+# few channels: one pass over the rows; a row, part of a wave's and of a workgroup's, several rounds of every workgroup
+NARROW = [(1, 8, 8), (15, 64, 128), (16, 128, 64), (17, 72, 120), (127, 64, 64), (128, 128, 128), (129, 8, 128), (300, 128, 8), (1000, 40, 56),
+          (32773, 24, 48), (70000, 128, 128), (70001, 64, 128), (33000, 128, 40)]
+
+
+@pytest.mark.parametrize("m,k,n", NARROW)
+@pytest.mark.parametrize("dtype", HALVES)
+def test_narrow_gradients(L, dtype, m, k, n):
+    for act in ACTS if m < 2000 else ("none", "relu", "gelu"):
+        check_gradients(L, act, dtype, m, k, n, m % 2 == 0)
+
+
+def test_narrow_pitches_and_alignments(either):
+    L = either
+    for lead, pad in ((0, 8), (1, 0), (3, 5), (8, 1)):
+        g = gen(pad)
+        rows = lambda r, c: normal(g, r * (c + pad) + lead)[lead:].view(r, c + pad)[:, :c]
+        x, w, b, dy = rows(400, 64), rows(104, 64), normal(g, 104 + lead)[lead:], rows(400, 104)
+        grads = lambda *t: torch.autograd.grad(L.linear(*t[:3], activation="silu"), t[:3], t[3])
+        want = grads(*[t.contiguous().clone().requires_grad_(i < 3) for i, t in enumerate((x, w, b, dy))])
+        got = grads(*[t.detach().requires_grad_(i < 3) for i, t in enumerate((x, w, b, dy))])
+        assert all(torch.equal(a, c) for a, c in zip(got, want)), (lead, pad)
+
+
+def test_narrow_not_numbers(L):
+    """An infinite weight whose products are positive: ReLU passes it, and what does not have to do with it stays finite -
+    the rows behind the last one are no rows, the channels behind the last one none either."""
+    g = gen(4)
+    for m, k, n in ((5, 64, 64), (131, 40, 24)):
+        x, w, dy = normal(g, m, k).abs(), normal(g, n, k), normal(g, m, n)
+        with torch.no_grad():
+            w[3, 7] = math.inf
+        x, w = x.requires_grad_(), w.requires_grad_()
+        b = torch.zeros(n, device="cuda", dtype=torch.float16, requires_grad=True)
+        gx, gw, gb = torch.autograd.grad(L.linear(x, w, b, activation="relu"), (x, w, b), dy)
+        assert gw.isfinite().all() and gb.isfinite().all()
+        want = R.mm(dy[:, 3:4].double().t(), x.detach().double().t())[0]
+        mag = R.mm(dy[:, 3:4].double().abs().t(), x.detach().double().t())[0]
+        within(gw[3], want, (m + 8) * 2.0 ** -23 * mag * 1.01 + half_step(want, torch.float16), "grad_weight")
+        assert gx[:, [i for i in range(k) if i != 7]].isfinite().all() and not gx[:, 7].isfinite().any()
+        x2 = x.detach().clone()
+        x2[2, 5] = math.nan
+        x2.requires_grad_()
+        gx, gw, gb = torch.autograd.grad(L.linear(x2, w.detach().nan_to_num(posinf=1.0).requires_grad_(), b, activation="gelu"), (x2, w, b), dy, allow_unused=True)[:3]
+        assert gx[2].isnan().all() and gx[[i for i in range(m) if i != 2]].isfinite().all() and gb.isnan().all()
+
+
+def test_narrow_beyond_two_gigabytes(L):
+    """Rows whose ends lie beyond 2^32 bytes."""
+    m, k, n = 36_000_000, 64, 64
+    x, dy = (torch.zeros(m, k, device="cuda", dtype=torch.float16) for _ in range(2))
+    x[-300:], dy[-300:] = normal(gen(1), 300, k), normal(gen(2), 300, n)
+    w = normal(gen(3), n, k, scale=1 / 8)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    gx, gw = torch.autograd.grad(L.linear(x, w, activation="silu"), leaves, dy)
+    with torch.no_grad():
+        tail, d = x[-300:].double(), dy[-300:].double()
+        dz = d * R.slope(R.mm(tail, w.double()), "silu", 0)
+        # the slope's error: that of the argument's sum and 2^-20; dz rounded; the sum of the products
+        ddz = d.abs() * (1.2 * sum_error(tail, w, k) + 2.0 ** -20) + half_step(dz, torch.float16)
+        mag = dz.abs() + ddz
+        want, aw = R.mm(dz, w.double().t()), w.double().abs().t()
+        within(gx[-300:], want, (R.mm(ddz, aw) + (n + 8) * 2.0 ** -23 * R.mm(mag, aw)) * (1 + EPS[torch.float16]) + half_step(want, torch.float16), "grad_x")
+        assert (gx[:-300] == 0).all()
+        want, ax = R.mm(dz.t(), tail.t()), tail.abs().t()
+        within(gw, want, (R.mm(ddz.t(), ax) + (300 + 8) * 2.0 ** -23 * R.mm(mag.t(), ax)) * (1 + EPS[torch.float16]) + half_step(want, torch.float16), "grad_weight")
+
+
+def test_narrow_writes_its_results_only(L):
+    import ctypes
+    from cumm_amd import _capi
+    g = gen(7)
+    for m, k, n in ((3, 40, 24), (129, 64, 72), (300, 128, 8)):
+        x, w, b, dy = normal(g, m, k), normal(g, n, k), normal(g, n), normal(g, m, n)
+        fields = [torch.full((size + 40,), 7.0, device="cuda", dtype=torch.float16) for size in (m * k, n * k, n)]
+        inner = [f[20:-20] for f in fields]
+        a = _capi.LinearGradArgs(dtype=7, m=m, n=n, k=k, grad_out=dy.data_ptr(), x=x.data_ptr(), weight=w.data_ptr(), bias=b.data_ptr(), ld_grad_out=n, ld_x=k,
+                                 ld_weight=k, grad_x=inner[0].data_ptr(), grad_weight=inner[1].data_ptr(), grad_bias=inner[2].data_ptr(), act_type=5, from_inputs=1)
+        need = _capi.lib().cumm_hip_linear_backward_workspace(ctypes.byref(a))
+        ws = torch.full((need + 512,), 7, dtype=torch.uint8, device="cuda")
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _capi.check(_capi.lib().cumm_hip_linear_backward(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
+        leaves = [t.requires_grad_() for t in (x, w, b)]
+        want = torch.autograd.grad(L.linear(*leaves, activation="gelu"), leaves, dy)
+        assert all(torch.equal(i.view_as(t), t) for i, t in zip(inner, want)) and (ws[need:] == 7).all()
+        for f, i in zip(fields, inner):
+            i.fill_(7.0)
+            assert (f == 7.0).all()
+
+
+def test_narrow_layers_keep_their_operands(either):
+    """What the activation got is worked out from the operands: one that was changed since is an error, as it is for any layer
+    that keeps an operand."""
+    L = either
+    for changed in ("x", "w", "b"):
+        t = dict(x=normal(gen(1), 40, 64).requires_grad_(), w=normal(gen(2), 32, 64), b=normal(gen(3), 32))
+        leaf = t["x"]
+        t["x"] = t["x"] * 1
+        out = L.linear(t["x"], t["w"], t["b"], activation="silu")
+        t[changed].add_(1)
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(out, leaf, torch.ones_like(out))
+
+
+@pytest.mark.parametrize("wanted", ["x", "w", "b", "xw", "wb", "xb"])
+def test_wide_some_gradients(either, wanted):
+    L = either
+    g = gen(5)
+    t = dict(x=normal(g, 90, 200), w=normal(g, 60, 200), b=normal(g, 60))
+    dy = normal(g, 90, 60)
+
+    def grads(names):
+        leaves = {k: v.detach().clone().requires_grad_(k in names) for k, v in t.items()}
+        out = L.linear(leaves["x"], leaves["w"], leaves["b"], activation="gelu")
+        return dict(zip(names, torch.autograd.grad(out, [leaves[k] for k in names], dy)))
+    all_of_them, some = grads("xwb"), grads(wanted)
+    for name in wanted:
+        assert torch.equal(some[name], all_of_them[name]), name
+
+
 @pytest.mark.parametrize("act", ["sigmoid", "leaky_relu", "silu", "gelu", "gelu_tanh"])
 def test_linear_gradient_against_differences(L, act):
     """The slope that the backward pass uses, against differences of the formula in 64 bits."""
@@ -554,6 +674,18 @@ def test_captured_training_step(either):
     def step(x, n, w, b, dy):
         out = L.linear(L.rms_norm(x, n), w, b, activation="gelu")
         return (out.detach(),) + torch.autograd.grad(out, (x, n, w, b), dy)
+    eager = lambda: step(*[v.detach().clone().requires_grad_(v.requires_grad) for v in t])
+    replays(lambda: step(*t), t, eager)
+
+
+def test_captured_narrow_training_step(either):
+    L = either
+    g = gen(2)
+    t = [normal(g, *s).requires_grad_() for s in ((700, 72), (104, 72), (104,))] + [normal(g, 700, 104)]
+
+    def step(x, w, b, dy):
+        out = L.linear(x, w, b, activation="gelu")
+        return (out.detach(),) + torch.autograd.grad(out, (x, w, b), dy)
     eager = lambda: step(*[v.detach().clone().requires_grad_(v.requires_grad) for v in t])
     replays(lambda: step(*t), t, eager)
 

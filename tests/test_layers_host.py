@@ -61,6 +61,10 @@ def test_linear_refuses(more, text):
     (dict(dtype=S8), "f16 or bf16"), (dict(n=0), "empty"), (dict(act_type=9), "activation"), (dict(ld_grad_out=63), "overlap"), (dict(ld_x=4 << 20), "8 MiB"),
     (dict(weight=None), "needs the weight"), (dict(x=None), "needs x"), (dict(grad_out=None), "null"), (dict(act_type=4), "pre_act"),
     (dict(grad_out=AT + 1), "aligned"), (dict(), "workspace"), (dict(m=(1 << 31) - 1, k=1 << 20, ld_x=1 << 20, ld_weight=1 << 20), "too many"),
+    (dict(from_inputs=1, n=60), "multiples of 8"), (dict(from_inputs=1, k=136, ld_x=136, ld_weight=136), "multiples of 8"),
+    (dict(from_inputs=1, n=136, ld_grad_out=136), "multiples of 8"), (dict(from_inputs=1, act_type=5, x=None, grad_weight=None), "x and weight"),
+    (dict(from_inputs=1, act_type=5, weight=None, grad_x=None), "x and weight"), (dict(from_inputs=1, bias=AT + 1), "aligned"),
+    (dict(from_inputs=1, grad_x=None, x=None), "needs x"), (dict(from_inputs=1, act_type=5), "workspace"),
 ])
 def test_linear_backward_refuses(more, text):
     refused(_capi.lib().cumm_hip_linear_backward, linear_grad(**more), text)
@@ -114,6 +118,9 @@ def test_workspaces():
     back = lambda **m: lib.cumm_hip_linear_backward_workspace(ctypes.byref(linear_grad(**dict(dict(grad_weight=None, grad_bias=None), **m))))
     plain = back()
     assert back(act_type=4, pre_act=AT, ld_pre_act=64) == plain + 100 * 64 * 2      # (100 rows of 64: 12800 bytes, 50 times 256)
+    narrow = back(from_inputs=1, act_type=4)
+    assert narrow == 64 * (128 + 1) * 4                         # one workgroup's sums: 100 rows are fewer than 128
+    assert back(from_inputs=1, act_type=4, m=129) == 2 * narrow and back(from_inputs=1, act_type=4, m=1 << 30) == 256 * narrow
     assert lib.cumm_hip_rms_norm_backward_workspace(ctypes.byref(norm_grad())) % (64 * 4) == 0
     assert lib.cumm_hip_rms_norm_backward_workspace(ctypes.byref(norm_grad(grad_weight=None))) == 0
 
