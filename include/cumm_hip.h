@@ -584,6 +584,7 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *args, void *stream);
  *   or, where codes is given instead of out, out in 8 bits: v = total * weight, top = the row's largest |v|, a code is the
  *   whole number next to 127 v / top (ties to even), scale = inv * top / 127 of the row: code * scale stands for out.
  *   weight NULL (with codes, without residual; dtype may then be CUMM_HIP_F32 too): rows in 8 bits without a norm, inv = 1.
+ *   Squares are added up in 32 bits: a bf16 row whose sum of them is above 3.4e38 has inv = 0 and so zeros.
  *   A row of zeros has codes 0 and scale 0; one with an infinity or a NaN has codes 0 and the scale that comes of it (an
  *   infinity or NaN), so that no wrong finite value results.  inv_rms [m], unless NULL, gets inv.  eps > 0.
  * cumm_hip_rms_norm_backward: for the gradients of out and of total (either NULL: zeros),

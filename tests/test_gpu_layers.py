@@ -305,6 +305,45 @@ def test_narrow_layers_keep_their_operands(either):
 
 
 @pytest.mark.parametrize("wanted", ["x", "w", "b", "xw", "wb", "xb"])
+@pytest.mark.parametrize("m,k,n", [(90, 40, 56), (200, 64, 128), (40, 200, 60)])
+def test_some_gradients_without_an_activation(either, wanted, m, k, n):
+    """Nothing is worked out again: an operand that no wanted gradient needs is not kept, and may change."""
+    L = either
+    g = gen(5)
+    t = dict(x=normal(g, m, k), w=normal(g, n, k), b=normal(g, n))
+    dy = normal(g, m, n)
+
+    def grads(names, change=()):
+        leaves = {k: v.detach().clone().requires_grad_(k in names) for k, v in t.items()}
+        out = L.linear(leaves["x"], leaves["w"], leaves["b"])
+        for name in change:
+            leaves[name].add_(1)
+        return dict(zip(names, torch.autograd.grad(out, [leaves[k] for k in names], dy)))
+    all_of_them = grads("xwb")
+    some = grads(wanted, "xw" if wanted == "b" else "")
+    for name in wanted:
+        assert torch.equal(some[name], all_of_them[name]), name
+
+
+def test_the_same_tensor_twice(either):
+    """x as its own residual, as its own weight, and under a norm as its own residual: the gradients add up."""
+    L = either
+    for c, act in ((64, "silu"), (200, "gelu")):
+        x, dy, w = normal(gen(1), c, c, scale=0.5), normal(gen(2), c, c), normal(gen(3), c, c, scale=c ** -0.5)
+        n = normal(gen(4), c)
+        one, two = x.clone().requires_grad_(), [x.clone().requires_grad_() for _ in range(2)]
+        got, = torch.autograd.grad(L.linear(one, w, activation=act, residual=one), one, dy)
+        parts = torch.autograd.grad(L.linear(two[0], w, activation=act, residual=two[1]), two, dy)
+        assert torch.equal(got, parts[0] + parts[1])
+        got, = torch.autograd.grad(L.linear(one, one, activation=act), one, dy)
+        parts = torch.autograd.grad(L.linear(two[0], two[1], activation=act), two, dy)
+        assert torch.equal(got, parts[0] + parts[1])
+        got, = torch.autograd.grad(L.rms_norm(one, n, residual=one), one, (dy, dy))
+        parts = torch.autograd.grad(L.rms_norm(two[0], n, residual=two[1]), two, (dy, dy))
+        assert torch.equal(got, parts[0] + parts[1])
+
+
+@pytest.mark.parametrize("wanted", ["x", "w", "b", "xw", "wb", "xb"])
 def test_wide_some_gradients(either, wanted):
     L = either
     g = gen(5)
