@@ -13,10 +13,12 @@ enum LinearLayout { kResult = 0, kGradInput = 1, kGradWeight = 2 };      // (XT,
 struct LinearPlan {
   int tile;      // kTile*
   int slices;
+  double us;     // its estimated time
 };
-enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5, kTile64Small = 6 };
+enum LinearTile { kTileFew = 0, kTile64 = 1, kTile64x128 = 2, kTile128 = 3, kTile128x256 = 4, kTile256 = 5, kTile64Small = 6, kTileAny = 7 };
 // k in units of two bytes
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k);
+LinearPlan linear_plan_any(const LinearPlan &plan, int64_t m, int n, int64_t k, int64_t copied);
 // whether its launch stays below 2^32 threads
 bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n);
 // bytes of the slices' sums (0 = one slice)

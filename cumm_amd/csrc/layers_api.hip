@@ -75,16 +75,22 @@ struct LinearCall {
   Operand x, weight;
   LinearPlan plan;
   int64_t k2;      // k in units of two bytes, as the copies have it
-  bool fits;
+  bool fits, any;  // any: the operands as they lie, whatever their alignment
   void *partial;
   LinearCall(const CummHipLinearArgs &a, Workspace &w) {
     const int size = a.dtype == CUMM_HIP_S8 ? 1 : 2;
     x = {a.x, a.m, a.k, a.ld_x, size};
     weight = {a.weight, a.n, a.k, a.ld_weight, size};
-    x.place(w);
-    weight.place(w);
     k2 = up((int64_t)a.k * size, 16) / 2;
     plan = linear_plan(kResult, a.m, a.n, k2);
+    if ((!x.direct() || !weight.direct()) && (int64_t)a.k * size >= 16) {      // (a piece lies inside its row)
+      plan = linear_plan_any(plan, a.m, a.n, k2, ((x.direct() ? 0 : x.rows) + (weight.direct() ? 0 : weight.rows)) * a.k * size);
+    }
+    any = plan.tile == kTileAny;
+    if (!any) {
+      x.place(w);
+      weight.place(w);
+    }
     fits = linear_plan_fits(plan, a.m, a.n);
     partial = plan.slices > 1 ? w.take(linear_partial_bytes(plan, a.m, a.n)) : nullptr;
   }
@@ -123,7 +129,7 @@ struct LinearGradCall {
   bool gated;              // a launch that writes dz, or the bias sums, or both
   const void *dz;
   int64_t ldz;             // elements
-  LinearPlan plan_x = {0, 1}, plan_w = {0, 1};
+  LinearPlan plan_x = {0, 1, 0}, plan_w = {0, 1, 0};
   void *partial_x = nullptr, *partial_w = nullptr;
   bool fits = true;
   LinearGradCall(const CummHipLinearGradArgs &a, Workspace &w) {
@@ -230,13 +236,14 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
   if (!call.fits) return bad(kTooMany);
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const hipError_t e = fill(call.x, call.weight, s);
+  const hipError_t e = call.any ? hipSuccess : fill(call.x, call.weight, s);
   if (e != hipSuccess) return launched(e);
   LinearParams p = {};
-  p.X = call.weight.at();
-  p.Y = call.x.at();
-  p.ldx = call.weight.pitch();
-  p.ldy = call.x.pitch();
+  p.X = call.any ? a->weight : call.weight.at();
+  p.Y = call.any ? a->x : call.x.at();
+  p.ldx = call.any ? a->ld_weight * call.x.bytes : call.weight.pitch();
+  p.ldy = call.any ? a->ld_x * call.x.bytes : call.x.pitch();
+  p.row_bytes = a->k * call.x.bytes;
   p.m = a->m;
   p.n = a->n;
   p.k = call.k2;

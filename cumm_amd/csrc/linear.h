@@ -10,6 +10,7 @@
 //   * addresses are 64 bits: a tile's descriptor begins at its own first row and moves by a step's bytes, so
 //     that no operand has a size limit; offsets inside a tile's step stay below 2^31 bytes (checked on the host);
 //   * 8-bit operands are pairs of bytes to the copies and the LDS layout, only the products know them;
+//   * operands that are not whole 16-byte pieces on 16-byte borders are copied, or read as they lie (linear_any_kernel);
 //   * the contraction can be cut into slices (grid.y), whose 32-bit sums a second kernel adds up in order;
 //   * the epilogue below.
 #pragma once
@@ -38,6 +39,7 @@ struct LinearParams {
   float slope;
   void *partial;           // slices > 1: [slices][m][n8] 32-bit sums, n8 = n rounded up to 8
   int32_t slices;
+  int32_t row_bytes;       // linear_any_kernel: k in bytes
 };
 
 // ---- the epilogue: values v[8] are consecutive columns n .. n + 7 of a row
@@ -749,6 +751,124 @@ __global__ __launch_bounds__(W * 64) void linear_few_kernel(const LinearParams p
     linear_columns<OUT, S8OP>(p, n, bias, scale);
     linear_finish8<OUT, S8OP, false>(p, m, n, v, bias, scale);
   }
+}
+
+// ---- rows as they lie, at any alignment: pieces of 16 bytes go through registers into LDS, SETS steps of them on their way, instead
+// of a copy of the operands and a launch for it.  Every load is made on every path (the compiler counts them): behind the end
+// of a row its last 16 bytes, which the last step shifts to where they belong, zeros behind them.  Loads at odd addresses bound
+// it, a quarter of the rate of aligned ones: 0.45 us a step for the 16 KB of a workgroup, with one step, three or four on the way
+// and with steps of 128 k all the same, 0.33 with several workgroups on the CU.  Whole words and the one behind them, put together in
+// registers, take longer (2001 x 1163 -> 777 20.4 us against 18.3: the words behind are as many loads again).
+template <int ROWS, int KS, int WAVES, int SLAB_BLOCKS, bool WIDE_ORDER>
+struct AnyOperand : DenseOperand<ROWS, KS, WAVES, false, SLAB_BLOCKS, WIDE_ORDER> {
+  using Base = DenseOperand<ROWS, KS, WAVES, false, SLAB_BLOCKS, WIDE_ORDER>;
+  const char *row[Base::IP];
+  int at[Base::IP];      // byte of the row
+
+  __device__ __forceinline__ void begin(int wave, int lane, const void *ptr, int64_t first, int64_t count, int64_t ld, int step) {
+#pragma unroll
+    for (int t = 0; t < Base::IP; ++t) {
+      const int slot = (wave * Base::IP + t) * 64 + lane;
+      const int rho = slot / Base::LPR, c = (slot % Base::LPR) ^ Base::swap_kc(rho);
+      const int i = rho & 15, nb = (rho >> 4) % SLAB_BLOCKS, slab = rho / (16 * SLAB_BLOCKS);
+      const int64_t r = first + (WIDE_ORDER ? slab * (16 * SLAB_BLOCKS) + (nb >> 1) * 32 + (i >> 2) * 8 + (nb & 1) * 4 + (i & 3) : rho);
+      row[t] = reinterpret_cast<const char *>(ptr) + (r < count ? r : count - 1) * ld;      // (rows behind the last are not stored)
+      at[t] = step * (Base::BK * 2) + c * 16;
+    }
+  }
+  __device__ __forceinline__ void load(v4i (&to)[Base::IP], int bytes) {
+#pragma unroll
+    for (int t = 0; t < Base::IP; ++t) {
+      to[t] = *reinterpret_cast<const v4i_any1 *>(row[t] + (at[t] < bytes - 16 ? at[t] : bytes - 16));
+      at[t] += Base::BK * 2;
+    }
+  }
+  // the pieces of the step `ahead` steps before the next load
+  __device__ __forceinline__ void store(char *lds, int wave, int lane, v4i (&from)[Base::IP], bool last, int ahead, int bytes) const {
+#pragma unroll
+    for (int t = 0; t < Base::IP; ++t) {
+      if (last) {
+        const int left = bytes - (at[t] - ahead * (Base::BK * 2)), bits = (16 - left) * 8;
+        if (left < 16) {
+          uint64_t lo = (uint32_t)from[t][0] | (uint64_t)(uint32_t)from[t][1] << 32, hi = (uint32_t)from[t][2] | (uint64_t)(uint32_t)from[t][3] << 32;
+          lo = left <= 0 ? 0 : (bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (64 - bits));
+          hi = left <= 8 ? 0 : hi >> bits;
+          from[t] = v4i{(int)(uint32_t)lo, (int)(uint32_t)(lo >> 32), (int)(uint32_t)hi, (int)(uint32_t)(hi >> 32)};
+        }
+      }
+      *reinterpret_cast<v4i *>(lds + ((wave * Base::IP + t) * 64 + lane) * 16) = from[t];
+    }
+  }
+};
+template <class T, class OUT, int WM, int WN, int RBW, int NBW, int KS, int SETS>
+__global__ __launch_bounds__(WM *WN * 64) void linear_any_kernel(const LinearParams p, int tiles_m, int tiles_n) {
+  using E = Elem<T>;
+  using AccV = typename E::AccV;
+  constexpr int TM = WM * RBW * 16, TN = WN * NBW * 16;
+  using OpY = AnyOperand<TM, KS, WM * WN, RBW, false>;
+  using OpX = AnyOperand<TN, KS, WM * WN, NBW, true>;
+  constexpr int STAGE = (OpY::VECS + OpX::VECS) * 16;
+  __shared__ __attribute__((aligned(16))) char ring[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+  int tile_m, tile_n;
+  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int64_t m0 = (int64_t)tile_m * TM;
+  const int n0 = tile_n * TN;
+  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  const int bytes = p.row_bytes, final = (bytes + OpY::BK * 2 - 1) / (OpY::BK * 2) - 1 - slice.first;      // the step that ends the rows
+  OpY y;
+  OpX x;
+  y.begin(wave, lane, p.Y, m0, p.m, p.ldy, slice.first);
+  x.begin(wave, lane, p.X, n0, p.n, p.ldx, slice.first);
+  int y_rd[KS], x_rd[KS];
+  y.offsets(lane, wm, y_rd);
+  x.offsets(lane, wn, x_rd);
+  AccV acc[RBW][NBW];
+#pragma unroll
+  for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+    for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = AccV{0, 0, 0, 0};
+  v4i ys[SETS][OpY::IP], xs[SETS][OpX::IP];
+#pragma unroll
+  for (int j = 0; j < SETS; ++j) {
+    y.load(ys[j], bytes);
+    x.load(xs[j], bytes);
+  }
+  for (int s0 = 0; s0 < slice.steps; s0 += SETS) {
+#pragma unroll
+    for (int j = 0; j < SETS; ++j) {
+      const int s = s0 + j;
+      if (s >= slice.steps) break;
+      // (a stage is written again two steps later: everybody has passed the barrier of the step between, and so read it)
+      char *st = ring + (s & 1) * STAGE;
+      y.store(st, wave, lane, ys[j], s == final, SETS, bytes);
+      x.store(st + OpY::VECS * 16, wave, lane, xs[j], s == final, SETS, bytes);
+      y.load(ys[j], bytes);
+      x.load(xs[j], bytes);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+      lds_barrier();
+      v4i yf[RBW][KS], xf[NBW][KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+#pragma unroll
+        for (int nb = 0; nb < NBW; ++nb) xf[nb][k] = OpX::fragment(st + OpY::VECS * 16, x_rd, k, nb);
+#pragma unroll
+        for (int rb = 0; rb < RBW; ++rb) yf[rb][k] = OpY::fragment(st, y_rd, k, rb);
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int rb = 0; rb < RBW; ++rb)
+#pragma unroll
+          for (int nb = 0; nb < NBW; ++nb) acc[rb][nb] = E::mfma(xf[nb][k], yf[rb][k], acc[rb][nb]);
+    }
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  lds_barrier();
+  constexpr int SHARE = 2 * STAGE / (WM * WN);
+  linear_epilogue<OUT, E::kBytes == 1, RBW, NBW, false, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
 }
 
 // The slices' sums added up, and the epilogue: eight columns of a row by LANES threads, which take every LANES-th slice in

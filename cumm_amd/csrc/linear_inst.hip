@@ -37,15 +37,17 @@ constexpr TileFigures kTiles[6][3] = {
     {{0, 8.813, 1.027, 0.04948, 0.4428, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}},      // 256 x 256
 };
 LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
-  if (layout == kResult && m <= 16) return {kTileFew, 1};
-  LinearPlan best = {kTile64, 1};
+  if (layout == kResult && m <= 16) {      // (the estimate: the wave's steps, or the weight at 4.8 TB/s)
+    return {kTileFew, 1, std::max(3.5 + 0.18 * (double)((k + 255) / 256), 2.0 + (double)n * k * 2e-6 / 4.8)};
+  }
+  LinearPlan best = {kTile64, 1, 0};
   double least = 1e300;
   const double operands = ((double)m * k + (double)n * k) * 2e-6, sums = (double)m * n * 4e-6;
   if (layout == kResult && m <= 64) {
     const bool two = m <= 32;      // blocks of 16 rows: two workgroups fit a CU, else one
     const double rounds = (double)(((n + 15) / 16 + (two ? 511 : 255)) / (two ? 512 : 256)), steps = (double)((k + 255) / 256);
     least = two ? 1.031 + rounds * (1.989 + 0.1778 * steps) : 1.397 + rounds * (2.037 + 0.2782 * steps);
-    best = {kTileFew, 1};
+    best = {kTileFew, 1, least};
   }
   constexpr int kShape[6][3] = {{64, 64, kTile64Small}, {64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);      // (more than fill the device many times over need no slices)
@@ -59,7 +61,7 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
       const TileFigures &f = kTiles[t][regime];
       const double us = f.launch + rounds * (f.turn + f.step * steps) + f.operands * (operands + (slices == 1 ? sums / 2 : 0.0)) +
                         (slices == 1 ? 0.0 : f.partial * sums * slices + f.join);
-      if (us < least) least = us, best = {kShape[t][2], slices};
+      if (us < least) least = us, best = {kShape[t][2], slices, us};
     }
   }
   return best;
@@ -74,8 +76,28 @@ bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n) {
   case kTile64x128: return threads(64, 128, 512);
   case kTile128: return threads(128, 128, 512);
   case kTile128x256: return threads(128, 256, 512);
+  case kTileAny: return threads(64, 64, 256);
   default: return threads(256, 256, 512);
   }
+}
+
+// The same for operands that are not whole pieces on 16-byte borders, `copied` bytes of them: the copy and the plan for its result, or
+// tiles that read them as they lie.  The copy costs a launch and what it moves; loads at odd addresses a step of 0.45 us where a
+// CU has one workgroup, 0.33 where it has more (aligned ones do not bound these tiles: 2001 x 1168 -> 777 12 – 13.6 us either way).  f16, with
+// the copy and as they lie: 1000 x 1001 -> 1000 14.1 us and 11.8, 15465 x 1603 -> 64 28.9 and 16.5, 5 x 2299 -> 6848 21.0 and 14.8 (two
+// slices), 64 x 999 -> 16000 20.9 and 12.4, 6 x 537 -> 64 10.6 and 7.3; 4000 x 3001 -> 2000 65 and 130, 1550 x 452 -> 8048 31 and 43.
+LinearPlan linear_plan_any(const LinearPlan &plan, int64_t m, int n, int64_t k, int64_t copied) {
+  LinearPlan best = plan;
+  best.us = plan.us + 4.0 + (double)copied * 2e-6 / 6.5;
+  const double sums = (double)m * n * 4e-6;
+  for (int slices = 1; slices <= 16 && (slices == 1 || k / slices >= 128); slices *= 2) {
+    const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
+    const int64_t wgs = (m + 63) / 64 * ((n + 63) / 64) * slices;
+    const double us = 3.3 + std::max(0.45 * steps, (double)((wgs + 255) / 256) * (0.33 * steps + 0.9)) + (slices == 1 ? 0.0 : 3.9 + 0.4 * sums * slices);
+    const LinearPlan any = {kTileAny, slices, us};
+    if (us < best.us && linear_plan_fits(any, m, n)) best = any;
+  }
+  return best;
 }
 
 hipError_t launch_linear_repack(LinearRepack p, int elem_bytes, hipStream_t s) {
@@ -157,6 +179,13 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
     else e = pipe<T, OUT, 4, 2, 2, XT, YT>(p, s);
     break;
   case kTile128x256: e = pipe<T, OUT, 4, 4, 3, XT, YT>(p, s); break;
+  case kTileAny:
+    if constexpr (!XT && !YT) {
+      const int tiles_m = (int)((p.m + 63) / 64), tiles_n = (p.n + 63) / 64;
+      hipLaunchKernelGGL((linear_any_kernel<T, OUT, 2, 2, 2, 2, 2, 2>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)p.slices), dim3(256), 0, s, p, tiles_m, tiles_n);
+      e = hipGetLastError();
+    }
+    break;
   case kTile256: e = large<T, OUT, XT, YT>(p, s); break;
   }
   return e == hipSuccess ? join<T, OUT>(p, s) : e;

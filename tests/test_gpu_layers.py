@@ -104,6 +104,39 @@ def test_linear_pitches_and_alignments(L, m, k, n, pad, lead):
     linear_case(L, torch.float16, m, k, n, "silu", True, True, seed=pad, pad=pad, lead=lead)
 
 
+# rows at any address, read as they lie (in slices of k too) or copied: ends of rows in each place of a piece, of a step, one step
+# after a slice; NaN around them
+@pytest.mark.parametrize("m,k,n", [(1, 8, 5), (1, 9, 64), (6, 63, 70), (64, 65, 64), (70, 127, 130), (20, 129, 33), (5, 2299, 700), (300, 8191, 300), (17, 4097, 260),
+                                   (2001, 191, 129), (3000, 193, 64), (16, 1025, 2050)])
+@pytest.mark.parametrize("kind", HALVES + [torch.int8])
+def test_linear_any_address(L, kind, m, k, n):
+    for lead in (1, 2, 3, 6) if m < 100 else (3,):
+        g = gen(lead)
+        dtype = torch.float16 if kind == torch.int8 else kind
+
+        def rows(r):
+            if kind == torch.int8:      # what lies around the rows would be seen in every sum
+                field = torch.full((r, k + 7), 127, device="cuda", dtype=torch.int8)
+                field[:, lead:lead + k] = torch.randint(-127, 128, (r, k), generator=g, device="cuda").to(torch.int8)
+            else:
+                field = torch.full((r, k + 7), math.nan, device="cuda", dtype=dtype)
+                field[:, lead:lead + k] = normal(g, r, k, dtype=dtype, scale=k ** -0.25)
+            return field[:, lead:lead + k]
+        x, w = rows(m), rows(n)
+        if kind == torch.int8:
+            xs, ws = torch.rand(m, generator=g, device="cuda") / 1000 + 1e-3, torch.rand(n, generator=g, device="cuda") / 1000 + 1e-3
+            got = L.linear_s8(x, xs, w, ws, dtype=dtype)
+            want = R.mm(x.double(), w.double()) * xs.double()[:, None] * ws.double()
+            # the sum to 32 bits and two products of it
+            within(got, want, want.abs() * 3 * 2.0 ** -24 * 1.01 + half_step(want, dtype) * 1.01, "linear_s8")
+        else:
+            b, r = normal(g, n, dtype=dtype), normal(g, m, n, dtype=dtype)
+            got = L.linear(x, w, b, residual=r)
+            _, want = R.linear(x, w, b, "none", r, 0)
+            err = sum_error(x, w, k) + (want - r.double()).abs() * 2.0 ** -23 + want.abs() * 2.0 ** -23
+            within(got, want, err * (1 + EPS[dtype]) + half_step(want, dtype), "linear")
+
+
 # every tile in every layout, whole and in slices: large, 128 x 256, 128 x 128 in two and three stages, ends of k inside steps
 @pytest.mark.parametrize("m,k,n", [(4093, 1000, 4088), (4093, 4088, 1000), (1000, 4088, 4093), (66000, 264, 680), (65272, 680, 168), (2040, 2056, 8200),
                                    (8200, 2040, 1030), (20000, 512, 520), (700, 20000, 500)])

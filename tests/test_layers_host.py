@@ -17,6 +17,10 @@ def linear(**more):
     return _capi.LinearArgs(**a)
 
 
+# operands that are copied: no whole pieces of 16 bytes, and products enough
+COPIED = dict(m=4000, n=4096, k=4095, ld_x=4096, ld_weight=4096, ld_out=4096)
+
+
 def linear_grad(**more):
     a = dict(dtype=F16, m=100, n=64, k=128, grad_out=AT, x=AT, weight=AT, ld_grad_out=64, ld_x=128, ld_weight=128, grad_x=AT, grad_weight=AT, grad_bias=AT)
     a.update(more)
@@ -49,7 +53,7 @@ def refused(fn, args, text):
     (dict(dtype=S8, x_scale=AT, weight_scale=AT, k=131072, ld_x=131072, ld_weight=131072), "131071"),
     (dict(dtype=S8, x_scale=AT, weight_scale=AT, bias=AT + 2), "aligned"), (dict(m=(1 << 31) - 1, n=1 << 20, ld_out=1 << 20), "too many"),
     (dict(m=16, n=(1 << 31) - 1, ld_out=(1 << 31) - 1), "too many"),
-    (dict(k=127, workspace=AT, workspace_bytes=10), "workspace"), (dict(k=127), "workspace"), (dict(k=127, workspace=AT + 16, workspace_bytes=1 << 30), "256-byte"),
+    (dict(COPIED, workspace=AT, workspace_bytes=10), "workspace"), (COPIED, "workspace"), (dict(COPIED, workspace=AT + 16, workspace_bytes=1 << 30), "256-byte"),
 ])
 def test_linear_refuses(more, text):
     refused(_capi.lib().cumm_hip_linear, linear(**more), text)
@@ -107,14 +111,16 @@ def test_no_rows_are_no_work():
 
 
 def test_workspaces():
-    """Operands that lie on 16-byte borders and are whole pieces long are read in place; others are copied to lines of 128
-    bytes; the gradient through an activation is kept for the two products."""
+    """Operands that lie on 16-byte borders and are whole pieces long are read in place; others too, or copied to lines of 128
+    bytes, whichever takes less time; the gradient through an activation is kept for the two products."""
     lib = _capi.lib()
     need = lambda **m: lib.cumm_hip_linear_workspace(ctypes.byref(linear(**m)))
     assert need(m=16) == 0
-    assert need(m=16, k=127) == 16 * 256 + 64 * 256             # both: 127 elements are no whole pieces
-    assert need(m=16, x=AT + 2) == 16 * 256                     # x alone
-    assert need(m=16, ld_weight=129) == 64 * 256
+    assert need(m=16, k=127) == need(m=16, x=AT + 2) == need(m=16, ld_weight=129) == 0
+    assert need(m=16, k=7) == 16 * 128 + 64 * 128               # (less than a piece)
+    assert need(**COPIED) == 4000 * 8192 + 4096 * 8192          # both: 4095 elements are no whole pieces
+    assert need(**dict(COPIED, k=4096, x=AT + 2)) == 4000 * 8192      # x alone
+    assert need(**dict(COPIED, k=4096, ld_weight=4097)) == 4096 * 8192
     back = lambda **m: lib.cumm_hip_linear_backward_workspace(ctypes.byref(linear_grad(**dict(dict(grad_weight=None, grad_bias=None), **m))))
     plain = back()
     assert back(act_type=4, pre_act=AT, ld_pre_act=64) == plain + 100 * 64 * 2      # (100 rows of 64: 12800 bytes, 50 times 256)
