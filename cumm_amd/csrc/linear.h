@@ -757,8 +757,9 @@ __global__ __launch_bounds__(W * 64) void linear_few_kernel(const LinearParams p
 // of a copy of the operands and a launch for it.  Every load is made on every path (the compiler counts them): behind the end
 // of a row its last 16 bytes, which the last step shifts to where they belong, zeros behind them.  Loads at odd addresses bound
 // it, a quarter of the rate of aligned ones: 0.45 us a step for the 16 KB of a workgroup, with one step, three or four on the way
-// and with steps of 128 k all the same, 0.33 with several workgroups on the CU.  Whole words and the one behind them, put together in
-// registers, take longer (2001 x 1163 -> 777 20.4 us against 18.3: the words behind are as many loads again).
+// and with steps of 128 k all the same, 0.33 with several workgroups on the CU.  Whole words, put together
+// in registers with the one behind them, take longer: 15465 x 1603 -> 64 20.2 us with a load for that word, 19.6 with the next lane's,
+// against 16.5.
 template <int ROWS, int KS, int WAVES, int SLAB_BLOCKS, bool WIDE_ORDER>
 struct AnyOperand : DenseOperand<ROWS, KS, WAVES, false, SLAB_BLOCKS, WIDE_ORDER> {
   using Base = DenseOperand<ROWS, KS, WAVES, false, SLAB_BLOCKS, WIDE_ORDER>;
