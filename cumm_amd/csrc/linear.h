@@ -386,6 +386,22 @@ __device__ __forceinline__ LinearSlice linear_slice(const LinearParams &p, int s
   return {first, end > first ? end - first : 0};
 }
 
+// Tile and slice of a workgroup: those that share an XCD take neighbouring tiles (as dense_tile has them) of the same slice
+__device__ __forceinline__ int linear_tile(int tiles_m, int tiles_n, int *tile_m, int *tile_n) {
+  const int tiles = (int)gridDim.x, all = tiles * (int)gridDim.y;
+  int logical = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+  if (all % 8 == 0) logical = logical % 8 * (all / 8) + logical / 8;
+  const int slice = logical / tiles;
+  logical -= slice * tiles;
+  constexpr int GROUP = 8;
+  const int per_group = GROUP * tiles_n;
+  const int g = logical / per_group, r = logical % per_group;
+  const int rows_here = tiles_m - g * GROUP < GROUP ? tiles_m - g * GROUP : GROUP;
+  *tile_m = g * GROUP + r % rows_here;
+  *tile_n = r / rows_here;
+  return slice;
+}
+
 // ---- tiles of WM x WN wave tiles times WK groups of waves that share a step's slices (densegemm_lds_kernel's loop)
 template <class T, class OUT, int WM, int WN, int WK, int RBW, int NBW, int KS, int NS, bool XT, bool YT>
 __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const LinearParams p, int tiles_m, int tiles_n) {
@@ -405,12 +421,12 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   const int wk = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
   constexpr int KW = KS / WK;
   int tile_m, tile_n;
-  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int of_slice = linear_tile(tiles_m, tiles_n, &tile_m, &tile_n);
   const int64_t m0 = (int64_t)tile_m * TM;
   const int n0 = tile_n * TN;
   OpY y;
   OpX x;
-  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  const LinearSlice slice = linear_slice(p, OpY::BK, of_slice);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
   int y_rd[YT ? RBW : KW], x_rd[XT ? NBW : KW];
@@ -458,7 +474,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
   lds_barrier();                          // and so has every other
   constexpr int SHARE = NS * STAGE / (WM * WN * WK);
   if constexpr (WK == 1) {
-    linear_epilogue<OUT, S8OP, RBW, NBW, XT, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
+    linear_epilogue<OUT, S8OP, RBW, NBW, XT, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, of_slice);
   } else {
     // each group finishes its share of the row blocks: it adds up all groups' sums of them, in group order
     constexpr int RO = RBW / WK;
@@ -482,7 +498,7 @@ __global__ __launch_bounds__(WM *WN *WK * 64) void linear_ring_kernel(const Line
       }
     __syncthreads();
     linear_epilogue<OUT, S8OP, RO, NBW, XT, false, SHARE>(p, own, m0 + wm * (RBW * 16) + wk * RO * 16, n0 + wn * (NBW * 16), lane,
-                                                          ring + wave * SHARE, (int)blockIdx.y);
+                                                          ring + wave * SHARE, of_slice);
   }
 }
 
@@ -506,12 +522,12 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
-  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int of_slice = linear_tile(tiles_m, tiles_n, &tile_m, &tile_n);
   const int64_t m0 = (int64_t)tile_m * TM;
   const int n0 = tile_n * TN;
   OpY y;
   OpX x;
-  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  const LinearSlice slice = linear_slice(p, OpY::BK, of_slice);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
   int y_rd[YT ? RBW : 2], x_rd[XT ? NBW : 2];
@@ -573,7 +589,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_pipe_kernel(const LinearPa
   __builtin_amdgcn_s_waitcnt(0xC07F);
   lds_barrier();
   constexpr int SHARE = NS * STAGE / (WM * WN);
-  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
+  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, of_slice);
 }
 
 // ---- the large tile: the same step, with loads and fragment reads dealt out among the products, a load per row block (all
@@ -597,12 +613,12 @@ __global__ __launch_bounds__(512) void linear_large_kernel(const LinearParams p,
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
-  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int of_slice = linear_tile(tiles_m, tiles_n, &tile_m, &tile_n);
   const int64_t m0 = (int64_t)tile_m * 256;
   const int n0 = tile_n * 256;
   OpY y;
   OpX x;
-  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  const LinearSlice slice = linear_slice(p, OpY::BK, of_slice);
   y.begin(wave, lane, p.Y, m0, p.m, p.ldy, p.k, slice.first);
   x.begin(wave, lane, p.X, n0, p.n, p.ldx, p.k, slice.first);
   int y_rd[YT ? RBW : 2], x_rd[XT ? NBW : 2];
@@ -668,7 +684,7 @@ __global__ __launch_bounds__(512) void linear_large_kernel(const LinearParams p,
   __builtin_amdgcn_s_waitcnt(0xC07F);
   lds_barrier();
   constexpr int SHARE = 2 * STAGE / 8;
-  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
+  linear_epilogue<OUT, S8OP, RBW, NBW, XT, true, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, of_slice);
 }
 
 // ---- few rows: MB blocks of 16 of them, 16 columns per workgroup, the steps dealt out to its W waves.  What counts is the
@@ -812,10 +828,10 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_any_kernel(const LinearPar
   __shared__ __attribute__((aligned(16))) char ring[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   int tile_m, tile_n;
-  dense_tile(tiles_m, tiles_n, &tile_m, &tile_n);
+  const int of_slice = linear_tile(tiles_m, tiles_n, &tile_m, &tile_n);
   const int64_t m0 = (int64_t)tile_m * TM;
   const int n0 = tile_n * TN;
-  const LinearSlice slice = linear_slice(p, OpY::BK, (int)blockIdx.y);
+  const LinearSlice slice = linear_slice(p, OpY::BK, of_slice);
   const int bytes = p.row_bytes, final = (bytes + OpY::BK * 2 - 1) / (OpY::BK * 2) - 1 - slice.first;      // the step that ends the rows
   OpY y;
   OpX x;
@@ -869,7 +885,7 @@ __global__ __launch_bounds__(WM *WN * 64) void linear_any_kernel(const LinearPar
   __builtin_amdgcn_s_waitcnt(0xC07F);
   lds_barrier();
   constexpr int SHARE = 2 * STAGE / (WM * WN);
-  linear_epilogue<OUT, E::kBytes == 1, RBW, NBW, false, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, (int)blockIdx.y);
+  linear_epilogue<OUT, E::kBytes == 1, RBW, NBW, false, false, SHARE>(p, acc, m0 + wm * (RBW * 16), n0 + wn * (NBW * 16), lane, ring + wave * SHARE, of_slice);
 }
 
 // The slices' sums added up, and the epilogue: eight columns of a row by LANES threads, which take every LANES-th slice in

@@ -19,7 +19,9 @@ namespace cummhip {
 // of 64 k.
 //   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
 // 64 x 64 in four waves and two stages (rows by the hundred thousand and a step or two: 119985 x 64 x 64 9.5 us against 12.7),
-// or in 2 x 2 x 2 waves and three; 64 x 128 in 2 x 4, three stages; the others through registers.  Few rows (17 to
+// or in 2 x 2 x 2 waves and three; 64 x 128 in 2 x 4, three stages; both with steps of 128 k where a CU has one workgroup (the figures
+// are those of 64 k: with smaller ones weight gradients choose these tiles, which read too much for them, 264 x 344 over 72024 rows 83 us);
+// the others through registers.  Few rows (17 to
 // 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
 // (31 x 2376 x 72 4.8 us against 14.1 in eight slices), above them while one round of workgroups does (60 x 5256 x 15680
 // 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 57 us in 64 slices of
@@ -161,6 +163,7 @@ static hipError_t few(const LinearParams &p, hipStream_t s) {
 template <class T, class OUT, bool XT, bool YT>
 static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, hipStream_t s) {
   hipError_t e = hipErrorInvalidValue;
+  const auto wgs = [&](int64_t tm, int tn) { return (p.m + tm - 1) / tm * ((p.n + tn - 1) / tn) * p.slices; };
   switch (plan.tile) {
   case kTileFew:
     if constexpr (!XT && !YT) {
@@ -172,10 +175,17 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
     }
     return e;
   case kTile64Small: e = ring<T, OUT, 2, 2, 1, 2, 2, 2, 2, XT, YT>(p, s); break;
-  case kTile64: e = ring<T, OUT, 2, 2, 2, 2, 2, 2, 3, XT, YT>(p, s); break;
-  case kTile64x128: e = ring<T, OUT, 2, 4, 1, 2, 2, 2, 3, XT, YT>(p, s); break;
+  // (one workgroup per CU: steps of 128 k, twice as much on its way: 1024 x 4096 x 1024 20.4 -> 16.0 us, 332 x 3648 x 1579 18.5 -> 15.7)
+  case kTile64:
+    if (wgs(64, 64) <= 256) e = ring<T, OUT, 2, 2, 2, 2, 2, 4, 4, XT, YT>(p, s);
+    else e = ring<T, OUT, 2, 2, 2, 2, 2, 2, 3, XT, YT>(p, s);
+    break;
+  case kTile64x128:
+    if (wgs(64, 128) <= 256) e = ring<T, OUT, 2, 4, 1, 2, 2, 4, 3, XT, YT>(p, s);
+    else e = ring<T, OUT, 2, 4, 1, 2, 2, 2, 3, XT, YT>(p, s);
+    break;
   case kTile128:      // (three stages where a CU has one workgroup: 2048^3 21.9 us against 24.9; two of two: 8192 x 1024 x 2048 39 against 48)
-    if (((p.m + 127) / 128) * ((p.n + 127) / 128) * p.slices <= 256) e = pipe<T, OUT, 4, 2, 3, XT, YT>(p, s);
+    if (wgs(128, 128) <= 256) e = pipe<T, OUT, 4, 2, 3, XT, YT>(p, s);
     else e = pipe<T, OUT, 4, 2, 2, XT, YT>(p, s);
     break;
   case kTile128x256: e = pipe<T, OUT, 4, 4, 3, XT, YT>(p, s); break;
