@@ -386,7 +386,9 @@ __device__ __forceinline__ LinearSlice linear_slice(const LinearParams &p, int s
   return {first, end > first ? end - first : 0};
 }
 
-// Tile and slice of a workgroup: those that share an XCD take neighbouring tiles (as dense_tile has them) of the same slice
+// Tile and slice of a workgroup: those that share an XCD take neighbouring tiles (as dense_tile has them) of the same slice, whose
+// rows its L2 then fetches once (dealt out among the XCDs by tile, weight gradients over many rows read them eight times: 256 x 256
+// over 100000 rows 50 us, so 31)
 __device__ __forceinline__ int linear_tile(int tiles_m, int tiles_n, int *tile_m, int *tile_n) {
   const int tiles = (int)gridDim.x, all = tiles * (int)gridDim.y;
   int logical = (int)(blockIdx.y * gridDim.x + blockIdx.x);
