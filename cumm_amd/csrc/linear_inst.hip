@@ -15,17 +15,15 @@ namespace cummhip {
 // Which kernel and how many slices: the least estimated time, in us on 256 CUs.  The figures are fitted (non-negative least
 // squares of the relative error, 12 % on average) to 42 k timings of 2400 random products of all three layouts, bf16: m to
 // 120000, n to 16384, k to 100000.  With them the choice is 4.6 % slower than the fastest of every kernel and number of
-// slices tried, on 1870 other products (fitted to those 4.2 %, but then 392 x 568 over 42200 rows takes 99 us instead of 46).  R: workgroups per CU, rounded up while there are one or two (one per CU: always), as they are beyond; steps
-// of 64 k.
+// slices tried, on 1870 other products (fitted to those 4.2 %, but then 392 x 568 over 42200 rows takes 99 us
+// instead of 46).  R: workgroups per CU, rounded up while there are one or two (one per CU: always), as they are beyond; steps of 64 k.
 //   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
 // 64 x 64 in four waves and two stages (rows by the hundred thousand and a step or two: 119985 x 64 x 64 9.5 us against 12.7),
 // or in 2 x 2 x 2 waves and three; 64 x 128 in 2 x 4, three stages; both with steps of 128 k where a CU has one workgroup; the others
-// through registers.  Few rows (17 to
-// 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
+// through registers.  Few rows (17 to 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
 // (31 x 2376 x 72 4.8 us against 14.1 in eight slices), above them while one round of workgroups does (60 x 5256 x 15680
-// 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 40 us in 16 of 64 x
-// 128); 128 x 256 where the large tile leaves half of the CUs idle (4096 x 8192 x
-// 2048 123 us, 128 x 128 142, 256 x 256 186); the large tile from about one per CU on (4096^3 103 us against 125).
+// 57 us against 31); slices where tiles leave CUs idle (weight gradient 264 x 344 over 72024 rows 40 us in 16 of 64 x 128);
+// 128 x 256 where the large tile leaves half of the CUs idle (4096 x 8192 x 2048 123 us, 128 x 128 142, 256 x 256 186); the large tile from about one per CU on (4096^3 103 us against 125).
 struct TileFigures {
   double launch, turn, step, operands, partial, join;
 };
