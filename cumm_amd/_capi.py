@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libcummhip.so")
 
 OK, EINVAL, ERUNTIME, ENOALGO = 0, 1, 2, 3
 LINEAR_NARROW = 128                # CUMM_HIP_LINEAR_NARROW
+LINEAR_GATE_BYTES = lambda n: 8 if n <= 64 else 16      # CUMM_HIP_LINEAR_GATE_BYTES
 STATIC_WORKSPACE_BYTES = 8 << 20   # CUMM_HIP_STATIC_WORKSPACE_BYTES
 
 
@@ -81,7 +82,7 @@ class LinearArgs(C.Structure):
                 ("out", C.c_void_p), ("pre_act", C.c_void_p), ("ld_x", C.c_int64), ("ld_weight", C.c_int64),
                 ("ld_residual", C.c_int64), ("ld_out", C.c_int64), ("ld_pre_act", C.c_int64), ("x_scale", C.c_void_p),
                 ("weight_scale", C.c_void_p), ("act_type", C.c_int32), ("act_alpha", C.c_float), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_size_t)]
+                ("workspace_bytes", C.c_size_t), ("gate", C.c_void_p)]
 
 
 class LinearGradArgs(C.Structure):
@@ -89,7 +90,8 @@ class LinearGradArgs(C.Structure):
                 ("pre_act", C.c_void_p), ("x", C.c_void_p), ("weight", C.c_void_p), ("ld_grad_out", C.c_int64),
                 ("ld_pre_act", C.c_int64), ("ld_x", C.c_int64), ("ld_weight", C.c_int64), ("grad_x", C.c_void_p),
                 ("grad_weight", C.c_void_p), ("grad_bias", C.c_void_p), ("act_type", C.c_int32), ("act_alpha", C.c_float),
-                ("from_inputs", C.c_int32), ("bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+                ("from_inputs", C.c_int32), ("bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("gate", C.c_void_p)]
 
 
 class RmsNormArgs(C.Structure):

@@ -50,10 +50,22 @@ struct LinearNarrowParams {
   const void *x, *grad, *weight, *bias;      // [rows, k], [rows, n], [n, k], [n] or NULL; x and weight NULL where nothing wants them
   void *grad_x, *grad_weight, *grad_bias;    // dense; each may be NULL
   float *partial;                            // linear_narrow_bytes
+  const void *gate;                          // of an activation with a kink, as the forward pass leaves it; NULL of any other
   int64_t rows, ldx, ldg, ldw;               // elements
   int32_t n, k, act;
   float slope;
 };
+// The forward pass of the same layers where the activation has a kink
+struct LinearNarrowForward {
+  const void *x, *weight, *bias, *residual;      // [rows, k], [n, k], [n] or NULL, [rows, n] or NULL
+  void *out, *pre, *gate;                        // [rows, n], [rows, n] and linear_narrow_gate_bytes; each may be NULL
+  int64_t rows, ldx, ldw, ldr, ldo, ldp;         // elements
+  int32_t n, k, act;
+  float slope;
+};
+int64_t linear_narrow_gate_bytes(int64_t rows, int n);
+bool linear_narrow_forward_takes(int n, int k, int act);
+hipError_t launch_linear_narrow_forward(const LinearNarrowForward &p, bool bf16, hipStream_t s);
 int64_t linear_narrow_bytes(int64_t rows, int n, int k);
 hipError_t launch_linear_narrow_backward(const LinearNarrowParams &p, bool bf16, hipStream_t s);
 // two-byte elements (a kernel: memset nodes of captured graphs have given wrong results on replays)

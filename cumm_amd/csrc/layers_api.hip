@@ -49,6 +49,10 @@ hipError_t fill(const Operand &a, const Operand &b, hipStream_t s) {
   return a.direct() && b.direct() ? hipSuccess : launch_linear_repack(LinearRepack{{a.repack(), b.repack()}}, a.bytes, s);
 }
 
+// Layers of few channels whose activation has a kink: rows and weight at any address, no workspace, and a gate for the backward pass
+bool narrow_forward(const CummHipLinearArgs &a) { return a.dtype != CUMM_HIP_S8 && linear_narrow_forward_takes(a.n, a.k, a.act_type); }
+bool narrow_gate(const CummHipLinearGradArgs &a) { return a.from_inputs && linear_narrow_forward_takes(a.n, a.k, a.act_type); }
+
 constexpr int kMaxRow = 1 << 30;                     // elements of a row of a norm
 
 const char *linear_checked(const CummHipLinearArgs &a) {
@@ -62,10 +66,11 @@ const char *linear_checked(const CummHipLinearArgs &a) {
   if (a.ld_x * size >= kRowBytes || a.ld_weight * size >= kRowBytes || up((int64_t)a.k * size, 128) >= kRowBytes) return "linear: rows of 8 MiB and more are not taken";
   if (s8 && a.k > kMaxWhole) return "linear: sums of more than 131071 products of 8 bits may exceed int32 range";
   if (a.act_type < 0 || a.act_type > CUMM_HIP_ACT_GELU_TANH) return "linear: unknown activation";
+  if (a.gate && !narrow_forward(a)) return "linear: a gate is left by two-byte layers of few channels with a ReLU or leaky ReLU";
   if (a.m == 0) return nullptr;
   if (!a.x || !a.weight || !a.out) return "linear: x, weight and out must not be null";
   if (s8 && (!a.x_scale || !a.weight_scale)) return "linear: 8-bit operands need the scales of their rows";
-  if (!on(a.x, size) || !on(a.weight, size) || !on(a.out, 2) || !on(a.residual, 2) || !on(a.pre_act, 2) || !on(a.bias, s8 ? 4 : 2) ||
+  if (!on(a.x, size) || !on(a.weight, size) || !on(a.out, 2) || !on(a.residual, 2) || !on(a.pre_act, 2) || !on(a.bias, s8 ? 4 : 2) || !on(a.gate, 4) ||
       (s8 && (!on(a.x_scale, 4) || !on(a.weight_scale, 4))))
     return "linear: a pointer is not aligned to its elements";
   return nullptr;
@@ -116,7 +121,11 @@ const char *linear_grad_checked(const CummHipLinearGradArgs &a) {
   if (!a.grad_out) return "linear backward: grad_out must not be null";
   if (a.from_inputs) {
     if (a.n % 8 || a.k % 8 || a.n > kLinearNarrow || a.k > kLinearNarrow) return "linear backward: from the inputs only where n and k are multiples of 8, up to 128";
-    if (a.act_type != CUMM_HIP_ACT_NONE && (!a.x || !a.weight)) return "linear backward: from the inputs, x and weight must not be null";
+    if (a.act_type != CUMM_HIP_ACT_NONE && !a.gate && (!a.x || !a.weight)) return "linear backward: from the inputs, x and weight must not be null";
+    if (a.gate && !narrow_gate(a)) return "linear backward: a gate is that of a ReLU or leaky ReLU";
+    if (!on(a.gate, 4)) return "linear backward: a pointer is not aligned to its elements";
+  } else if (a.gate) {
+    return "linear backward: a gate goes with from_inputs";
   } else if (a.act_type != CUMM_HIP_ACT_NONE && !a.pre_act) return "linear backward: the activation's argument (pre_act) is missing";
   for (const void *p : {a.grad_out, a.pre_act, a.x, a.weight, a.bias, (const void *)a.grad_x, (const void *)a.grad_weight, (const void *)a.grad_bias})
     if (!on(p, 2)) return "linear backward: a pointer is not aligned to its elements";
@@ -221,7 +230,7 @@ extern "C" {
 
 int64_t cumm_hip_linear_workspace(const CummHipLinearArgs *a) {
   if (!a || linear_checked(*a)) return -1;
-  if (a->m == 0) return 0;
+  if (a->m == 0 || narrow_forward(*a)) return 0;
   Workspace w = {nullptr};
   const LinearCall call(*a, w);
   return call.fits ? w.used : -1;
@@ -231,11 +240,16 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
   if (!a) return bad("linear: null arguments");
   if (const char *e = linear_checked(*a)) return bad(e);
   if (a->m == 0) return CUMM_HIP_OK;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (narrow_forward(*a)) {
+    const LinearNarrowForward p = {a->x, a->weight, a->bias, a->residual, a->out, a->pre_act, a->gate, a->m, a->ld_x, a->ld_weight, a->ld_residual,
+                                   a->ld_out, a->ld_pre_act, a->n, a->k, a->act_type, a->act_alpha};
+    return launched(launch_linear_narrow_forward(p, a->dtype == CUMM_HIP_BF16, s));
+  }
   Workspace w = {reinterpret_cast<char *>(a->workspace)};
   const LinearCall call(*a, w);
   if (!call.fits) return bad(kTooMany);
   if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, w.used)) return bad(e);
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hipError_t e = call.any ? hipSuccess : fill(call.x, call.weight, s);
   if (e != hipSuccess) return launched(e);
   LinearParams p = {};
@@ -267,7 +281,9 @@ int cumm_hip_linear(const CummHipLinearArgs *a, void *stream) {
 int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *a) {
   if (!a || linear_grad_checked(*a)) return -1;
   if (a->m == 0) return 0;
-  if (a->from_inputs) return up(linear_narrow_bytes(a->m, a->n, a->k), 256);
+  if (a->from_inputs) {
+    return up(linear_narrow_bytes(a->m, a->n, a->k), 256) + (narrow_gate(*a) && !a->gate ? up(linear_narrow_gate_bytes(a->m, a->n), 256) : 0);
+  }
   Workspace w = {nullptr};
   const LinearGradCall call(*a, w);
   return call.fits ? w.used : -1;
@@ -285,9 +301,18 @@ int cumm_hip_linear_backward(const CummHipLinearGradArgs *a, void *stream) {
   if (a->from_inputs) {
     if (const char *e = workspace_checked(a->workspace, a->workspace_bytes, cumm_hip_linear_backward_workspace(a))) return bad(e);
     if (!a->grad_x && !a->grad_weight && !a->grad_bias) return CUMM_HIP_OK;
+    const bool bf16 = a->dtype == CUMM_HIP_BF16;
+    const void *gate = a->gate;
+    if (narrow_gate(*a) && !gate) {      // nobody has kept it: a forward pass for it alone
+      void *made = reinterpret_cast<char *>(a->workspace) + up(linear_narrow_bytes(a->m, a->n, a->k), 256);
+      const LinearNarrowForward p = {a->x, a->weight, a->bias, nullptr, nullptr, nullptr, made, a->m, a->ld_x, a->ld_weight, 0, 0, 0, a->n, a->k, a->act_type, a->act_alpha};
+      const hipError_t e = launch_linear_narrow_forward(p, bf16, s);
+      if (e != hipSuccess) return launched(e);
+      gate = made;
+    }
     const LinearNarrowParams p = {a->x, a->grad_out, a->weight, a->bias, a->grad_x, a->grad_weight, a->grad_bias, reinterpret_cast<float *>(a->workspace),
-                                  a->m, a->ld_x, a->ld_grad_out, a->ld_weight, a->n, a->k, a->act_type, a->act_alpha};
-    return launched(launch_linear_narrow_backward(p, a->dtype == CUMM_HIP_BF16, s));
+                                  gate, a->m, a->ld_x, a->ld_grad_out, a->ld_weight, a->n, a->k, a->act_type, a->act_alpha};
+    return launched(launch_linear_narrow_backward(p, bf16, s));
   }
   Workspace w = {reinterpret_cast<char *>(a->workspace)};
   const LinearGradCall call(*a, w);

@@ -58,7 +58,7 @@ int layer_type(at::ScalarType t) { return t == at::kChar ? CUMM_HIP_S8 : (t == a
 
 // out, and what the activation got (undefined unless wanted); scales: of 8-bit operands
 std::pair<Tensor, Tensor> linear_result(const Tensor &x_, const Tensor &w_, const Tensor &bias, const Tensor &residual, int64_t act, double slope, at::ScalarType out_type,
-                                        bool want_pre, const Tensor &x_scale, const Tensor &w_scale) {
+                                        bool want_pre, const Tensor &x_scale, const Tensor &w_scale, const Tensor &gate = Tensor()) {
   const Rows x(x_), w(w_);
   const c10::Device device = x_.device();
   const auto options = kind_of(out_type, device);
@@ -84,6 +84,7 @@ std::pair<Tensor, Tensor> linear_result(const Tensor &x_, const Tensor &w_, cons
     a.ld_residual = r.pitch;
   }
   if (want_pre) a.pre_act = pre.data_ptr();
+  if (gate.defined()) a.gate = gate.data_ptr();
   if (x_scale.defined()) {
     a.x_scale = (xs = x_scale.contiguous()).data_ptr<float>();
     a.weight_scale = (ws = w_scale.contiguous()).data_ptr<float>();
@@ -109,14 +110,16 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_,
                         const std::optional<Tensor> &residual_, int64_t act, double slope, bool save_x, bool save_w) {
     const Tensor bias = given(bias_), residual = given(residual_);
-    // what the activation got: of few channels worked out again in the backward pass; the sign of a ReLU's result is that of
-    // its argument, unless something is added to it
+    // what the backward pass needs of the activation's argument.  Of few channels it is worked out again, or, where only its side of a
+    // kink counts, kept as a bit; the sign of a ReLU's result is that of its argument, unless something is added to it
     const auto narrow = [](int64_t c) { return c % 8 == 0 && c <= CUMM_HIP_LINEAR_NARROW; };
-    const bool again = narrow(w.size(0)) && narrow(w.size(1)), whole = again && act != CUMM_HIP_ACT_NONE;
+    const bool again = narrow(w.size(0)) && narrow(w.size(1)), kink = again && (act == CUMM_HIP_ACT_RELU || act == CUMM_HIP_ACT_LEAKY_RELU);
+    const bool whole = again && act != CUMM_HIP_ACT_NONE && !kink;
     const bool by_result = act == CUMM_HIP_ACT_RELU && !residual.defined() && !again;
     const bool keep = act != CUMM_HIP_ACT_NONE && !by_result && !again;
-    const auto got = linear_result(x, w, bias, residual, act, slope, x.scalar_type(), keep, Tensor(), Tensor());
-    ctx->save_for_backward({save_x || whole ? x : Tensor(), save_w || whole ? w : Tensor(), whole ? bias : (by_result ? got.first : got.second)});
+    const Tensor gate = kink ? bytes(x.numel() / x.size(-1) * CUMM_HIP_LINEAR_GATE_BYTES(w.size(0)), x.device()) : Tensor();
+    const auto got = linear_result(x, w, bias, residual, act, slope, x.scalar_type(), keep, Tensor(), Tensor(), gate);
+    ctx->save_for_backward({save_x || whole ? x : Tensor(), save_w || whole ? w : Tensor(), kink ? gate : (whole ? bias : (by_result ? got.first : got.second))});
     ctx->saved_data["again"] = again;
     ctx->saved_data["edges"] = (int64_t)(bias.defined() ? 1 : 0) | (residual.defined() ? 2 : 0);
     ctx->saved_data["act"] = act;
@@ -149,7 +152,9 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
       a.ld_grad_out = g.pitch;
       Tensor bias;
       a.from_inputs = ctx->saved_data["again"].toBool();
-      if (saved[2].defined() && a.from_inputs) {
+      if (saved[2].defined() && a.from_inputs && saved[2].scalar_type() == at::kByte) {
+        a.gate = saved[2].data_ptr();
+      } else if (saved[2].defined() && a.from_inputs) {
         a.bias = (bias = saved[2].contiguous()).data_ptr();
       } else if (saved[2].defined()) {
         a.pre_act = saved[2].data_ptr();

@@ -19,6 +19,7 @@ from . import tensorview as tv
 
 ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "leaky_relu": 3, "silu": 4, "gelu": 5, "gelu_tanh": 6}
 _TYPES = {torch.float16: int(tv.float16), torch.bfloat16: int(tv.bfloat16), torch.int8: int(tv.int8), torch.float32: int(tv.float32)}
+_KINKS = (ACTIVATIONS["relu"], ACTIVATIONS["leaky_relu"])
 _HALVES = (torch.float16, torch.bfloat16)
 
 
@@ -93,7 +94,7 @@ def _call(fn, query, args, device) -> None:
 
 # ---- linear
 
-def _linear_forward(x, weight, bias, residual, act, slope, scales, dtype, want_pre):
+def _linear_forward(x, weight, bias, residual, act, slope, scales, dtype, want_pre, gate=None):
     """(out, pre_act or None) for matrices."""
     lib = _capi.lib()
     m, k, n = x.shape[0], x.shape[1], weight.shape[0]
@@ -103,7 +104,7 @@ def _linear_forward(x, weight, bias, residual, act, slope, scales, dtype, want_p
         a = _capi.LinearArgs()
         a.dtype, a.out_dtype, a.m, a.n, a.k = _TYPES[x.dtype], _TYPES[dtype], m, n, k
         a.x, a.weight, a.bias, a.residual = x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual)
-        a.out, a.pre_act = out.data_ptr(), _ptr(pre)
+        a.out, a.pre_act, a.gate = out.data_ptr(), _ptr(pre), _ptr(gate)
         a.ld_x, a.ld_weight, a.ld_out, a.ld_pre_act = _pitch(x), _pitch(weight), n, n
         if residual is not None:
             a.ld_residual = _pitch(residual)
@@ -118,15 +119,19 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act: int, slope: float):
-        # what the activation got: of few channels worked out again in the backward pass; the sign of a ReLU's result is that of
-        # its argument, unless something is added to it
+        # what the backward pass needs of the activation's argument.  Of few channels it is worked out again, or, where only its side
+        # of a kink counts, kept as a bit; the sign of a ReLU's result is that of its argument, unless something is added to it
         ctx.again = all(c % 8 == 0 and c <= _capi.LINEAR_NARROW for c in weight.shape)
-        whole = ctx.again and act != 0
+        ctx.kink = ctx.again and act in _KINKS
+        whole = ctx.again and act != 0 and not ctx.kink
         by_result = act == ACTIVATIONS["relu"] and residual is None and not ctx.again
-        out, pre = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, act != 0 and not by_result and not ctx.again)
+        gate = None
+        if ctx.kink:
+            gate = torch.empty(x.shape[0], _capi.LINEAR_GATE_BYTES(weight.shape[0]), dtype=torch.uint8, device=x.device)
+        out, pre = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, act != 0 and not by_result and not ctx.again, gate)
         ctx.act, ctx.slope, ctx.n = act, slope, weight.shape[0]
         ctx.save_for_backward(x if ctx.needs_input_grad[1] or whole else None, weight if ctx.needs_input_grad[0] or whole else None,
-                              bias if whole else (out if by_result else pre))
+                              gate if ctx.kink else (bias if whole else (out if by_result else pre)))
         return out
 
     @staticmethod
@@ -143,7 +148,9 @@ class _Linear(torch.autograd.Function):
                 a = _capi.LinearGradArgs()
                 a.dtype, a.m, a.n, a.k, a.grad_out, a.ld_grad_out = _TYPES[g.dtype], m, n, k, g.data_ptr(), _pitch(g)
                 a.from_inputs = ctx.again
-                if pre is not None and ctx.again:
+                if ctx.kink:
+                    a.gate = pre.data_ptr()
+                elif pre is not None and ctx.again:
                     a.bias = pre.data_ptr()
                 elif pre is not None:
                     a.pre_act, a.ld_pre_act = pre.data_ptr(), n
@@ -188,7 +195,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None, slope: float = 0.01) -> torch.Tensor:
     """``act(x @ weight.T + bias) + residual`` for x [..., K], weight [N, K] (f16 / bf16); one rounding.  Differentiable in
     all four tensors (once); with N and K multiples of 8 up to 128, the backward pass works out what the activation got from x,
-    weight and bias, which are kept for that.  ``slope`` is that of "leaky_relu"."""
+    weight and bias, which are kept for that, or, for "relu" and "leaky_relu", keeps which elements pass, a bit each, decided by the
+    exact sign of the activation's argument.  ``slope`` is that of "leaky_relu"."""
     native = _native()
     if native is not None and activation in ACTIVATIONS:
         out = native.layer_linear(x, weight, bias, residual, ACTIVATIONS[activation], slope)

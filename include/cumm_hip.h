@@ -537,13 +537,19 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
  *   pre_act, unless NULL, gets what the activation gets (rounded): the backward pass wants it.
  *   out may be residual itself, with its pitch; apart from that no output overlaps an operand.
  *   m == 0 is no work; NaN passes through every activation.
+ *   ReLU and leaky ReLU of f16 / bf16 layers with n and k multiples of 8 up to CUMM_HIP_LINEAR_NARROW: an argument that 32 bits cannot
+ *   tell from zero is added up in 64, so that its sign is right, and gate, unless NULL (it is for these layers only, 4-byte aligned), gets
+ *   which elements of the gradient pass, for the backward pass to read.
  * cumm_hip_linear_backward: the gradients for grad_out [m, n], each NULL where it is not wanted:
  *     dz = grad_out act'(pre_act);  grad_x = dz weight [m, k];  grad_weight = dz^T x [n, k];  grad_bias = sum of dz's rows
  *   (the residual's is grad_out).  dz is rounded to dtype for the two products, not for the sum.  pre_act NULL: only with
  *   CUMM_HIP_ACT_NONE; for CUMM_HIP_ACT_RELU without a residual, out serves as well.  m == 0 gives zeros.
  *   from_inputs != 0, for n and k that are multiples of 8 up to CUMM_HIP_LINEAR_NARROW: one pass over the rows that works
- *   out what the activation got from x, weight and bias ([n] or NULL; an activation needs the first two); pre_act is not read. */
+ *   out what the activation got from x, weight and bias ([n] or NULL; an activation needs the first two); pre_act is not read.
+ *   With a ReLU or leaky ReLU, what passes is read from gate, as the forward pass has left it (an element whose argument is not above
+ *   zero does not, a NaN passes; x, weight and bias are not needed for it then), or, where that is NULL, worked out in a launch before. */
 #define CUMM_HIP_LINEAR_NARROW 128
+#define CUMM_HIP_LINEAR_GATE_BYTES(n) ((n) <= 64 ? 8 : 16)
 #define CUMM_HIP_ACT_SILU 4
 #define CUMM_HIP_ACT_GELU 5        /* x Phi(x), by erf */
 #define CUMM_HIP_ACT_GELU_TANH 6
@@ -559,6 +565,7 @@ typedef struct CummHipLinearArgs {
   float act_alpha;                               /* slope of CUMM_HIP_ACT_LEAKY_RELU */
   void *workspace;
   size_t workspace_bytes;
+  void *gate;                                    /* [m] rows of CUMM_HIP_LINEAR_GATE_BYTES(n), or NULL */
 } CummHipLinearArgs;
 int64_t cumm_hip_linear_workspace(const CummHipLinearArgs *args);
 int cumm_hip_linear(const CummHipLinearArgs *args, void *stream);
@@ -575,6 +582,7 @@ typedef struct CummHipLinearGradArgs {
   const void *bias;
   void *workspace;
   size_t workspace_bytes;
+  const void *gate;
 } CummHipLinearGradArgs;
 int64_t cumm_hip_linear_backward_workspace(const CummHipLinearGradArgs *args);
 int cumm_hip_linear_backward(const CummHipLinearGradArgs *args, void *stream);
