@@ -111,7 +111,9 @@ __device__ __forceinline__ float linear_act_slope(float z, int act, float slope)
   }
   case kActSilu: {
     const float p = logistic_of_exponent(-kLog2e * z);
-    return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+    // (beyond |z| = 128 p is 0 or 1; an infinite z - any that the type it is kept in cannot hold - would be infinity times zero)
+    const float zc = __builtin_amdgcn_fmed3f(z, -128.0f, 128.0f);
+    return p * __builtin_fmaf(zc, 1.0f - p, 1.0f);
   }
   case kActGeluTanh: {
     const float p = logistic_of_exponent(-z * __builtin_fmaf(kGeluB, z * z, kGeluA));

@@ -1,0 +1,49 @@
+"""Gradients of the row-wise layers' activations where numbers leave their type's range (``cumm_amd.torch_layers``)."""
+import math
+
+import pytest
+import torch
+
+import layers_ref as R
+
+pytestmark = pytest.mark.gpu
+
+ACTS = ["none", "relu", "sigmoid", "leaky_relu", "silu", "gelu", "gelu_tanh"]
+
+
+@pytest.fixture(scope="module")
+def L():
+    from cumm_amd import torch_bridge, torch_layers
+    assert torch_bridge._native() is not None
+    return torch_layers
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("n", [64, 136])      # few channels, and more, whose argument is kept in f16
+@pytest.mark.parametrize("residual", [False, True])
+def test_slopes_of_arguments_beyond_the_type(L, act, n, residual):
+    """Arguments of +-90000, finite in 32 bits and infinite in f16: the slopes there are 0, 1 or the leak, whether the gradient that
+    comes is zero or not, and the channels beside are as ever."""
+    m, k, leak = 40, 8, 0.25
+    x, w = torch.zeros(m, k, device="cuda", dtype=torch.float16), torch.zeros(n, k, device="cuda", dtype=torch.float16)
+    x[:, 0], x[:, 1] = 60000, 1
+    sign = torch.where(torch.arange(n, device="cuda") % 2 == 0, 1.0, -1.0)
+    w[:, 0], w[n // 2:, 0], w[:, 1] = 1.5 * sign, 0, 0.5 * sign      # half of the channels are ordinary: +-0.5
+    dy = torch.zeros(m, n, device="cuda", dtype=torch.float16)
+    dy[:5] = 2.0 ** -8
+    r = torch.zeros(m, n, device="cuda", dtype=torch.float16) if residual else None
+    b = torch.zeros(n, device="cuda", dtype=torch.float16)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(L.linear(*leaves, activation=act, residual=r, slope=leak), leaves, dy)
+    with torch.no_grad():
+        z = R.mm(x.double(), w.double())
+        far = z.abs() > 1e4
+        slope = R.slope(torch.where(far, z.sign() * 700, z), act, leak)      # (as at infinity)
+        dz = dy.double() * slope
+        # a slope is off by 2^-20, its product with the gradient rounded once, sums in 32 bits, rounded once; halves of the smallest step
+        ddz = dy.double() * 2.0 ** -20 + dz.abs() * 2.0 ** -11 + 2.0 ** -25
+        ax, aw = x.double(), w.double().abs()
+        want = R.mm(dz, w.double().t()), R.mm(dz.t(), x.double().t()), dz.sum(0)
+        errs = R.mm(ddz, aw.t()), R.mm(ddz.t(), ax.t()), ddz.sum(0)
+        for name, a, e, err in zip(("grad_x", "grad_weight", "grad_bias"), got, want, errs):
+            assert ((a.double() - e).abs() <= err * 1.01 + e.abs() * (2.0 ** -11 + 2.0 ** -16) + 2.0 ** -25).all(), name
