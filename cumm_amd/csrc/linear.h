@@ -100,11 +100,9 @@ __device__ __forceinline__ void linear_act(float (&v)[N], int act, float slope) 
   }
 }
 
-// the derivative of the activation where its argument is z
-__device__ __forceinline__ float linear_act_slope(float z, int act, float slope) {
+// the derivative of a smooth activation where its argument is z
+__device__ __forceinline__ float linear_act_slope(float z, int act) {
   switch (act) {
-  case kActRelu: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-  case kActLeakyRelu: return z > 0.0f ? 1.0f : (z != z ? z : slope);
   case kActSigmoid: {
     const float p = logistic_of_exponent(-kLog2e * z);
     return p * (1.0f - p);
@@ -133,15 +131,22 @@ __device__ __forceinline__ float linear_act_slope(float z, int act, float slope)
   }
 }
 
-// Eight of them, multiplied into g: one branch for all
+// Eight of them, multiplied into g: one branch for all.  Those with a kink choose: where nothing passes there is no product, an
+// infinite gradient times zero is not NaN; the gradient of an argument that is NaN passes.
 __device__ __forceinline__ void linear_act_slopes(float (&g)[8], const v4f &lo, const v4f &hi, int act, float slope) {
   const auto all = [&](auto one) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] *= linear_act_slope(e < 4 ? lo[e] : hi[e - 4], decltype(one)::value, slope);
+    for (int e = 0; e < 8; ++e) g[e] *= linear_act_slope(e < 4 ? lo[e] : hi[e - 4], decltype(one)::value);
   };
   switch (act) {
-  case kActRelu: all(std::integral_constant<int, kActRelu>{}); break;
-  case kActLeakyRelu: all(std::integral_constant<int, kActLeakyRelu>{}); break;
+  case kActRelu:
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = (e < 4 ? lo[e] : hi[e - 4]) <= 0.0f ? 0.0f : g[e];
+    break;
+  case kActLeakyRelu:
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = (e < 4 ? lo[e] : hi[e - 4]) <= 0.0f ? g[e] * slope : g[e];
+    break;
   case kActSigmoid: all(std::integral_constant<int, kActSigmoid>{}); break;
   case kActSilu: all(std::integral_constant<int, kActSilu>{}); break;
   case kActGelu: all(std::integral_constant<int, kActGelu>{}); break;

@@ -542,12 +542,13 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
  *   which elements of the gradient pass, for the backward pass to read.
  * cumm_hip_linear_backward: the gradients for grad_out [m, n], each NULL where it is not wanted:
  *     dz = grad_out act'(pre_act);  grad_x = dz weight [m, k];  grad_weight = dz^T x [n, k];  grad_bias = sum of dz's rows
- *   (the residual's is grad_out).  dz is rounded to dtype for the two products, not for the sum.  pre_act NULL: only with
+ *   (the residual's is grad_out).  A ReLU's dz is grad_out itself or zero, that of an argument that is NaN the former; leaky likewise.
+ *   dz is rounded to dtype for the two products, not for the sum.  pre_act NULL: only with
  *   CUMM_HIP_ACT_NONE; for CUMM_HIP_ACT_RELU without a residual, out serves as well.  m == 0 gives zeros.
  *   from_inputs != 0, for n and k that are multiples of 8 up to CUMM_HIP_LINEAR_NARROW: one pass over the rows that works
  *   out what the activation got from x, weight and bias ([n] or NULL; an activation needs the first two); pre_act is not read.
- *   With a ReLU or leaky ReLU, what passes is read from gate, as the forward pass has left it (an element whose argument is not above
- *   zero does not, a NaN passes; x, weight and bias are not needed for it then), or, where that is NULL, worked out in a launch before. */
+ *   With a ReLU or leaky ReLU, what passes is read from gate, as the forward pass has left it (x, weight and bias are not needed for it
+ *   then), or, where that is NULL, worked out in a launch before. */
 #define CUMM_HIP_LINEAR_NARROW 128
 #define CUMM_HIP_LINEAR_GATE_BYTES(n) ((n) <= 64 ? 8 : 16)
 #define CUMM_HIP_ACT_SILU 4

@@ -47,3 +47,33 @@ def test_slopes_of_arguments_beyond_the_type(L, act, n, residual):
         errs = R.mm(ddz, aw.t()), R.mm(ddz.t(), ax.t()), ddz.sum(0)
         for name, a, e, err in zip(("grad_x", "grad_weight", "grad_bias"), got, want, errs):
             assert ((a.double() - e).abs() <= err * 1.01 + e.abs() * (2.0 ** -11 + 2.0 ** -16) + 2.0 ** -25).all(), name
+
+
+@pytest.mark.parametrize("act", ["relu", "leaky_relu"])
+@pytest.mark.parametrize("n", [64, 136])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("python", [False, True])
+def test_infinite_gradients_stop_at_a_gate(L, monkeypatch, act, n, residual, python):
+    """A gradient that is infinite (an overflow of scaled losses) is zero behind a closed ReLU, the leak times it behind a leaky one; one
+    of an argument that is NaN passes."""
+    if python:
+        from cumm_amd import torch_bridge
+        monkeypatch.setattr(torch_bridge, "_native_module", False)
+    m, k, leak = 12, 8, 0.25
+    x, w = (torch.zeros(r, k, device="cuda", dtype=torch.float16) for r in (m, n))
+    x[:, 0] = torch.where(torch.arange(m, device="cuda") % 2 == 0, 1.0, -1.0)
+    x[9, 0] = math.nan
+    w[:, 0], w[:, 1] = 1, 2.0 ** -9
+    b = torch.zeros(n, device="cuda", dtype=torch.float16)
+    dy = torch.ones(m, n, device="cuda", dtype=torch.float16)
+    dy[3, 5] = dy[4, 6] = math.inf      # behind a closed gate, and an open one
+    r = torch.zeros(m, n, device="cuda", dtype=torch.float16) if residual else None
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    gx, _, gb = torch.autograd.grad(L.linear(*leaves, activation=act, residual=r, slope=leak), leaves, dy)
+    off = 0.0 if act == "relu" else leak
+    rows = [i for i in range(m) if i not in (3, 4)]
+    passes = torch.where(torch.arange(m, device="cuda") % 2 == 0, 1.0, off)
+    passes[9] = 1
+    assert torch.equal(gx[rows, 1], (passes[rows] * n * 2.0 ** -9).half())
+    assert float(gx[4, 1]) == math.inf and float(gx[3, 1]) == (0 if act == "relu" else math.inf)
+    assert float(gb[6]) == math.inf and (act == "leaky_relu" or bool(gb[5].isfinite()))
