@@ -6,9 +6,11 @@ each, and the product of such rows.  Every computing kernel, of the gradients to
 Tensors are f16 or bf16 on one GPU, of any number of leading dimensions; the last one is the row.  Rows may be any number of
 elements apart; a tensor whose rows are not contiguous, or whose leading dimensions are not one run of rows, is copied.
 Calls go to the current stream of the tensors' device and allocate from torch's caching allocator: they can be captured
-into graphs.  A failed check raises ValueError, a failed launch RuntimeError.
+into graphs.  ``torch.jit.trace`` records a call as a Python operator; forward-mode derivatives and make_fx, which would see the
+allocations and not the launch, are refused.  A failed check raises ValueError, a failed launch RuntimeError.
 """
 import ctypes
+import sys
 from typing import Optional, Tuple, Union
 
 import torch
@@ -34,6 +36,34 @@ def _native():
     if torch._C._are_functorch_transforms_active() or torch.compiler.is_compiling():
         return None
     return torch_bridge._native()
+
+
+def _not_recorded(name: str, *tensors) -> None:
+    """Refuses what would leave the launch out and say nothing: a derivative in forward mode, a graph of torch's operators."""
+    if torch.autograd.forward_ad._current_level >= 0 and any(
+            t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("%s has no derivative in forward mode" % name)
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if proxies is not None and proxies.get_proxy_mode() is not None:
+        raise ValueError("%s cannot be recorded as torch operators" % name)
+
+
+def _differentiable(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _Recorded(torch.autograd.Function):
+    """A call without a gradient where ``torch.jit.trace`` records: a Python operator in its graph."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        out = fn(*args)
+        ctx.mark_non_differentiable(*(out if isinstance(out, tuple) else (out,)))
+        return out
+
+
+def _made(fn, *args):
+    return _Recorded.apply(fn, *args) if torch.jit.is_tracing() else fn(*args)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -113,6 +143,10 @@ def _linear_forward(x, weight, bias, residual, act, slope, scales, dtype, want_p
         a.act_type, a.act_alpha = act, slope
         _call(lib.cumm_hip_linear, lib.cumm_hip_linear_workspace, a, x.device)
     return out, pre
+
+
+def _linear_result(x, weight, bias, residual, act, slope, x_scale, weight_scale, dtype):
+    return _linear_forward(x, weight, bias, residual, act, slope, None if x_scale is None else (x_scale, weight_scale), dtype, False)[0]
 
 
 class _Linear(torch.autograd.Function):
@@ -202,13 +236,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         out = native.layer_linear(x, weight, bias, residual, ACTIVATIONS[activation], slope)
         if out is not None:
             return out
+    _not_recorded("linear", x, weight, bias, residual)
     _check(x.dtype in _HALVES, "linear: x must be float16 or bfloat16 (linear_s8 takes 8-bit rows)")
     shape = x.shape[:-1] + weight.shape[:1]
     x, weight, bias, residual, act = _linear_args("linear", x, weight, bias, residual, activation, x.dtype, x.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _differentiable(x, weight, bias, residual):
         out = _Linear.apply(x, weight, bias, residual, act, slope)
     else:
-        out = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, False)[0]
+        out = _made(_linear_result, x, weight, bias, residual, act, slope, None, None, x.dtype)
     return out if out.shape == shape else out.view(shape)
 
 
@@ -230,11 +265,9 @@ def linear_s8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     _check(weight_scale.dtype == torch.float32 and weight_scale.shape == weight.shape[:1],
            "linear_s8: weight_scale must be float32, one per row of weight")
     _on_device(x, x_scale=x_scale, weight_scale=weight_scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, weight_scale, bias, residual)):
-        raise ValueError("linear_s8 has no gradient: call it under torch.no_grad()")
+    _no_gradient("linear_s8", x_scale, weight_scale, bias, residual)
     x, weight, bias, residual, act = _linear_args("linear_s8", x, weight, bias, residual, activation, dtype, torch.float32)
-    out, _ = _linear_forward(x, weight, bias, residual, act, slope, (x_scale.contiguous(), weight_scale.contiguous()), dtype, False)
-    return out.view(shape)
+    return _made(_linear_result, x, weight, bias, residual, act, slope, x_scale.contiguous(), weight_scale.contiguous(), dtype).view(shape)
 
 
 # ---- norms
@@ -261,6 +294,12 @@ def _norm_forward(x, weight, residual, eps, codes: bool, want_inv: bool):
         a.inv_rms = _ptr(inv)
         _call(lib.cumm_hip_rms_norm, None, a, x.device)
     return out, scale, total, inv
+
+
+def _norm_result(x, weight, residual, eps, codes):
+    """What the caller gets: out or codes, then scale and total where there are."""
+    got = tuple(t for t in _norm_forward(x, weight, residual, eps, codes, False)[:3] if t is not None)
+    return got if len(got) > 1 else got[0]
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -321,13 +360,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
         got = native.layer_norm(x, weight, residual, eps, False)
         if got is not None:
             return got
+    _not_recorded("rms_norm", x, weight, residual)
     shape = x.shape
     x, weight, residual = _norm_args("rms_norm", x, weight, residual, eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _differentiable(x, weight, residual):
         got = _RmsNorm.apply(x, weight, residual, eps)
     else:
-        out, _, total, _ = _norm_forward(x, weight, residual, eps, False, False)
-        got = out if total is None else (out, total)
+        got = _made(_norm_result, x, weight, residual, eps, False)
     if residual is None:
         return got.view(shape)
     return got[0].view(shape), got[1].view(shape)
@@ -345,9 +384,8 @@ def rms_norm_s8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, res
     _no_gradient("rms_norm_s8", x, weight, residual)
     shape = x.shape
     x, weight, residual = _norm_args("rms_norm_s8", x, weight, residual, eps)
-    codes, scale, total, _ = _norm_forward(x, weight, residual, eps, True, False)
-    got = codes.view(shape), scale.view(shape[:-1])
-    return got if total is None else got + (total.view(shape),)
+    codes, scale, *total = _made(_norm_result, x, weight, residual, eps, True)
+    return (codes.view(shape), scale.view(shape[:-1])) + tuple(t.view(shape) for t in total)
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -363,12 +401,13 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _check(x.dtype in _HALVES or x.dtype == torch.float32, "quantize_rows: x must be float16, bfloat16 or float32")
     _on_device(x)
     shape = x.shape
-    codes, scale, _, _ = _norm_forward(_rows(x), None, None, 1.0, True, False)
+    codes, scale = _made(_norm_result, _rows(x), None, None, 1.0, True)
     return codes.view(shape), scale.view(shape[:-1])
 
 
 def _no_gradient(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    _not_recorded(name, *tensors)
+    if _differentiable(*tensors):
         raise ValueError("%s has no gradient: call it under torch.no_grad()" % name)
 
 
