@@ -3,6 +3,7 @@
 // forward-mode derivatives - is left to the Python functions, which say what is wrong or do the same; a call that this
 // file makes has their results.  Part of torch_native.cpp.
 #pragma once
+#include <algorithm>
 
 // tensors that these calls take as they are
 bool simple(const Tensor &t, const c10::Device &device, at::ScalarType type) {
@@ -105,6 +106,13 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads) {
   return (*error)(std::move(marked));
 }
 
+// A tensor that was kept for the backward pass, as it comes back: an unpack hook may give another one
+const Tensor &kept(const Tensor &t, const char *name, const c10::Device &device, at::ScalarType type, c10::IntArrayRef sizes) {
+  TORCH_CHECK_VALUE(t.defined() && simple(t, device, type) && t.sizes() == sizes, "the tensor kept as ", name, " came back as ", t.toString(), " ", t.sizes(), " on ", t.device(),
+                    ", not as ", type, " ", sizes, " on ", device);
+  return t;
+}
+
 struct LinearLayer : torch::autograd::Function<LinearLayer> {
   // (a tensor that is not there has no edge in the graph: its gradient's place is counted in `edges`)
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &bias_,
@@ -147,35 +155,40 @@ struct LinearLayer : torch::autograd::Function<LinearLayer> {
       a.dtype = layer_type(grad.scalar_type());
       a.m = g.rows;
       a.n = (int32_t)g.cols;
-      a.k = 8;
       a.grad_out = g.at();
       a.ld_grad_out = g.pitch;
-      Tensor bias;
+      const at::ScalarType type = grad.scalar_type();
+      const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
       a.from_inputs = ctx->saved_data["again"].toBool();
-      if (saved[2].defined() && a.from_inputs && saved[2].scalar_type() == at::kByte) {
-        a.gate = saved[2].data_ptr();
-      } else if (saved[2].defined() && a.from_inputs) {
-        a.bias = (bias = saved[2].contiguous()).data_ptr();
-      } else if (saved[2].defined()) {
-        a.pre_act = saved[2].data_ptr();
-        a.ld_pre_act = g.cols;
-      }
       a.act_type = (int32_t)ctx->saved_data["act"].toInt();
       a.act_alpha = (float)ctx->saved_data["slope"].toDouble();
+      a.k = (int32_t)shape.back();
+      Tensor third;
+      Rows pre;
+      if (saved[2].defined() && a.from_inputs && (a.act_type == CUMM_HIP_ACT_RELU || a.act_type == CUMM_HIP_ACT_LEAKY_RELU)) {
+        const int64_t bytes = std::max<int64_t>(g.rows * CUMM_HIP_LINEAR_GATE_BYTES(g.cols), 256);
+        a.gate = (third = kept(saved[2], "gate", device, at::kByte, {bytes}).contiguous()).data_ptr();
+      } else if (saved[2].defined() && a.from_inputs) {
+        a.bias = (third = kept(saved[2], "bias", device, type, {g.cols}).contiguous()).data_ptr();
+      } else if (saved[2].defined()) {
+        // (the result has the call's leading dimensions, what the activation got has one)
+        third = saved[2].dim() == 2 ? saved[2] : saved[2].detach().reshape({-1, saved[2].size(-1)});
+        pre = Rows(kept(third, "the activation's argument", device, type, {g.rows, g.cols}));
+        a.pre_act = pre.at();
+        a.ld_pre_act = pre.pitch;
+      }
       if (saved[1].defined()) {
-        w = Rows(saved[1]);
-        a.k = (int32_t)w.cols;
+        w = Rows(kept(saved[1], "weight", device, type, {g.cols, shape.back()}));
         a.weight = w.at();
         a.ld_weight = w.pitch;
       }
       if (saved[0].defined()) {
-        x = Rows(saved[0]);
-        a.k = (int32_t)x.cols;
+        x = Rows(kept(saved[0], "x", device, type, shape));
         a.x = x.at();
         a.ld_x = x.pitch;
       }
       if (need[0]) {
-        result[0] = at::empty(ctx->saved_data["shape"].toIntVector(), options);
+        result[0] = at::empty(shape, options);
         a.grad_x = result[0].data_ptr();
       }
       if (need[1]) {
@@ -284,10 +297,12 @@ struct NormLayer : torch::autograd::Function<NormLayer> {
     const auto saved = ctx->get_saved_variables();
     {
       at::AutoGradMode no_grad(false);
-      const c10::Device device = saved[0].device();
+      const Tensor &any = grad.defined() ? grad : grad_total;      // (of the result's shape and type, as x)
+      const c10::Device device = any.device();
       const c10::DeviceGuard guard(device);
-      const Rows h(saved[0].detach());
-      const Tensor w = saved[1].detach().contiguous();
+      const Rows h(kept(saved[0], "the normed rows", device, any.scalar_type(), any.sizes()).detach());
+      const Tensor w = kept(saved[1], "weight", device, any.scalar_type(), {h.cols}).detach().contiguous();
+      const Tensor inv = kept(saved[2], "the rows' statistics", device, at::kFloat, {h.rows}).contiguous();
       Rows g, t;
       Tensor grad_x;
       CummHipRmsNormGradArgs a = {};
@@ -297,7 +312,7 @@ struct NormLayer : torch::autograd::Function<NormLayer> {
       a.total = h.at();
       a.ld_total = h.pitch;
       a.weight = w.data_ptr();
-      a.inv_rms = saved[2].data_ptr<float>();
+      a.inv_rms = inv.data_ptr<float>();
       if (grad.defined()) {
         g = Rows(grad.detach());
         a.grad_out = g.at();

@@ -86,6 +86,13 @@ def _on_device(first: torch.Tensor, **others) -> None:
             raise ValueError("%s is on %s, not on %s" % (name, t.device, first.device))
 
 
+def _kept(name: str, t: torch.Tensor, like: torch.Tensor, dtype, *shape) -> torch.Tensor:
+    """A tensor that was kept for the backward pass, as it comes back: an unpack hook may give another one."""
+    _check(t.device == like.device and t.dtype == dtype and t.shape == shape,
+           "the tensor kept as %s came back as %s %s on %s, not as %s %s on %s" % (name, t.dtype, tuple(t.shape), t.device, dtype, shape, like.device))
+    return t
+
+
 class _Device:
     """The device of a call's tensors, where it is not the current one."""
 
@@ -163,7 +170,7 @@ class _Linear(torch.autograd.Function):
         if ctx.kink:
             gate = torch.empty(x.shape[0], _capi.LINEAR_GATE_BYTES(weight.shape[0]), dtype=torch.uint8, device=x.device)
         out, pre = _linear_forward(x, weight, bias, residual, act, slope, None, x.dtype, act != 0 and not by_result and not ctx.again, gate)
-        ctx.act, ctx.slope, ctx.n = act, slope, weight.shape[0]
+        ctx.act, ctx.slope, ctx.k = act, slope, weight.shape[1]
         ctx.save_for_backward(x if ctx.needs_input_grad[1] or whole else None, weight if ctx.needs_input_grad[0] or whole else None,
                               gate if ctx.kink else (bias if whole else (out if by_result else pre)))
         return out
@@ -177,21 +184,26 @@ class _Linear(torch.autograd.Function):
         if need_x or need_w or need_b:
             lib, g = _capi.lib(), _rows(grad)
             m, n = g.shape
-            k = next((t.shape[1] for t in (x, weight) if t is not None), 8)
+            k = ctx.k
             with _Device(g.device):
                 a = _capi.LinearGradArgs()
                 a.dtype, a.m, a.n, a.k, a.grad_out, a.ld_grad_out = _TYPES[g.dtype], m, n, k, g.data_ptr(), _pitch(g)
                 a.from_inputs = ctx.again
                 if ctx.kink:
+                    pre = _kept("gate", pre, g, torch.uint8, m, _capi.LINEAR_GATE_BYTES(n)).contiguous()
                     a.gate = pre.data_ptr()
                 elif pre is not None and ctx.again:
+                    pre = _kept("bias", pre, g, g.dtype, n).contiguous()
                     a.bias = pre.data_ptr()
                 elif pre is not None:
-                    a.pre_act, a.ld_pre_act = pre.data_ptr(), n
+                    pre = _rows(_kept("the activation's argument", pre, g, g.dtype, m, n))
+                    a.pre_act, a.ld_pre_act = pre.data_ptr(), _pitch(pre)
                 a.act_type, a.act_alpha = ctx.act, ctx.slope
                 if x is not None:
+                    x = _rows(_kept("x", x, g, g.dtype, m, k))
                     a.x, a.ld_x = x.data_ptr(), _pitch(x)
                 if weight is not None:
+                    weight = _rows(_kept("weight", weight, g, g.dtype, n, k))
                     a.weight, a.ld_weight = weight.data_ptr(), _pitch(weight)
                 if need_x:
                     grad_x = torch.empty((m, k), dtype=g.dtype, device=g.device)
@@ -316,7 +328,13 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, grad, grad_total=None):
         total, weight, inv = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        m, k = total.shape
+        if grad is None and grad_total is None:
+            return None, None, None, None
+        like = grad if grad is not None else grad_total      # (of the result's shape and type, as x)
+        m, k = like.shape
+        total = _rows(_kept("the normed rows", total, like, like.dtype, m, k))
+        weight = _kept("weight", weight, like, like.dtype, k).contiguous()
+        inv = _kept("the rows' statistics", inv, like, torch.float32, m).contiguous()
         lib = _capi.lib()
         grad_x = grad_w = None
         with _Device(total.device):
