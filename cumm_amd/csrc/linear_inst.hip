@@ -35,25 +35,32 @@ constexpr TileFigures kTiles[6][3] = {
     {{0, 6.656, 0.6827, 0.03557, 0.576, 0.845}, {3.231, 4.953, 0.794, 0.02276, 0.2717, 0}, {3.231, 4.953, 0.794, 0.02276, 0.2717, 0}},      // 128 x 256
     {{0, 8.813, 1.027, 0.04948, 0.4428, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}, {0, 5.446, 1.354, 0.03894, 0.3245, 0}},      // 256 x 256
 };
-LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
-  if (layout == kResult && m <= 16) {      // (the estimate: the wave's steps, or the weight at 4.8 TB/s)
+// Kernels whose launch would have too many threads are passed over; where all would, the plan is one that does not fit.
+LinearPlan linear_plan(LinearLayout layout, int64_t m, int n_, int64_t k) {
+  const int64_t n = n_;      // (the sums below may pass 2^31)
+  const LinearPlan few = {kTileFew, 1, 0};
+  const bool few_fit = linear_plan_fits(few, m, n_);
+  if (layout == kResult && m <= 16 && few_fit) {      // (the estimate: the wave's steps, or the weight at 4.8 TB/s)
     return {kTileFew, 1, std::max(3.5 + 0.18 * (double)((k + 255) / 256), 2.0 + (double)n * k * 2e-6 / 4.8)};
   }
   LinearPlan best = {kTile64, 1, 0};
   double least = 1e300;
   const double operands = ((double)m * k + (double)n * k) * 2e-6, sums = (double)m * n * 4e-6;
-  if (layout == kResult && m <= 64) {
+  if (layout == kResult && m <= 64 && few_fit) {
     const bool two = m <= 32;      // blocks of 16 rows: two workgroups fit a CU, else one
     const double rounds = (double)(((n + 15) / 16 + (two ? 511 : 255)) / (two ? 512 : 256)), steps = (double)((k + 255) / 256);
     least = two ? 1.031 + rounds * (1.989 + 0.1778 * steps) : 1.397 + rounds * (2.037 + 0.2782 * steps);
     best = {kTileFew, 1, least};
   }
   constexpr int kShape[6][3] = {{64, 64, kTile64Small}, {64, 64, kTile64}, {64, 128, kTile64x128}, {128, 128, kTile128}, {128, 256, kTile128x256}, {256, 256, kTile256}};
+  bool fits[6];
+  for (int t = 0; t < 6; ++t) fits[t] = linear_plan_fits({kShape[t][2], 1, 0}, m, n_);
   const int64_t tiles = ((m + 63) / 64) * ((n + 63) / 64);      // (more than fill the device many times over need no slices)
   for (int slices = 1; slices <= 256; slices *= 2) {
     if (slices > 1 && (k / slices < 128 || tiles * slices > 16384)) break;
     const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
     for (int t = 0; t < 6; ++t) {
+      if (!fits[t]) continue;
       const double wgs = (double)((m + kShape[t][0] - 1) / kShape[t][0]) * (double)((n + kShape[t][1] - 1) / kShape[t][1]) * slices;
       const int regime = wgs <= 256 ? 0 : (wgs <= 512 ? 1 : 2);
       const double rounds = regime < 2 ? regime + 1.0 : (t >= 4 ? (double)(int64_t)((wgs + 255) / 256) : wgs / 256);
@@ -69,7 +76,7 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n, int64_t k) {
 bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n) {
   const auto threads = [&](int64_t tm, int64_t tn, int64_t per) { return (m + tm - 1) / tm * ((n + tn - 1) / tn) * per < (int64_t)1 << 32; };
   switch (plan.tile) {
-  case kTileFew: return threads(m, 16, 512);
+  case kTileFew: return threads(m, 16, m > 16 ? 256 : (n >= 8192 ? 128 : 512));
   case kTile64Small: return threads(64, 64, 256);
   case kTile64: return threads(64, 64, 512);
   case kTile64x128: return threads(64, 128, 512);
@@ -91,7 +98,7 @@ LinearPlan linear_plan_any(const LinearPlan &plan, int64_t m, int n, int64_t k, 
   const double sums = (double)m * n * 4e-6;
   for (int slices = 1; slices <= 16 && (slices == 1 || k / slices >= 128); slices *= 2) {
     const double steps = (double)(((k + slices - 1) / slices + 63) / 64);
-    const int64_t wgs = (m + 63) / 64 * ((n + 63) / 64) * slices;
+    const int64_t wgs = (m + 63) / 64 * (((int64_t)n + 63) / 64) * slices;
     const double us = 3.3 + std::max(0.45 * steps, (double)((wgs + 255) / 256) * (0.33 * steps + 0.9)) + (slices == 1 ? 0.0 : 3.9 + 0.4 * sums * slices);
     const LinearPlan any = {kTileAny, slices, us};
     if (us < best.us && linear_plan_fits(any, m, n)) best = any;

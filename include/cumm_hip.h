@@ -527,8 +527,9 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
  * sum and applies the activation to both, and its int8 inference epilogue takes scales that somebody has made.
  * Types f16 and bf16 (dtype), and what each entry names beside them; every sum, norm and scale is 32 bits, every result is
  * rounded once.  Rows may be any number of elements apart (ld*), at any alignment of an element; operands whose rows do
- * not lie on 16-byte borders, or are no multiple of 16 bytes long, are copied into the workspace first where that pays.  Rows of m up to
- * 2^31 - 1, of less than 8 MiB each; nothing else is limited.  Nothing is allocated, no stream waited for; calls that may
+ * not lie on 16-byte borders, or are no multiple of 16 bytes long, are copied into the workspace first where that pays.  Up to 2^31 - 1
+ * rows; those of a product's operands are of less than 8 MiB each, and its result has less than 2^23 tiles of 256 x 256, ends of rows and columns
+ * counted whole; those of a norm have up to 2^30 elements.  Nothing is allocated, no stream waited for; calls that may
  * overlap in time need a workspace each (*_workspace bytes, 256-byte aligned; -1 for arguments that are not taken).
  *
  * cumm_hip_linear:  out[r][c] = act(sum_k x[r][k] weight[c][k] + bias[c]) + residual[r][c]

@@ -1,0 +1,46 @@
+"""Row-wise layers of sizes near the limits of a launch."""
+import pytest
+import torch
+
+import layers_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def L():
+    from cumm_amd import torch_bridge, torch_layers
+    assert torch_bridge._native() is not None
+    return torch_layers
+
+
+def whole(g, *shape):
+    return torch.randint(-3, 4, shape, generator=g, device="cuda", dtype=torch.int8).half()
+
+
+@pytest.mark.parametrize("m", [1, 17])
+def test_linear_of_very_many_columns(L, m):
+    """2^27 of them: whole numbers, so that every sum is exact."""
+    n, k = 1 << 27, 8
+    g = torch.Generator(device="cuda").manual_seed(m)
+    x, w = whole(g, m, k), whole(g, n, k)
+    if m > 1:
+        n = (1 << 26) + 40
+        w = w[:n]
+    got = L.linear(x, w)
+    for row in range(0, m, 8):
+        want = torch.zeros(n, device="cuda")
+        for j in range(k):
+            want += x[row, j].float() * w[:, j].float()
+        assert torch.equal(got[row], want.half())
+
+
+def test_linear_of_very_many_rows(L):
+    m, n, k = (1 << 30) + 77, 8, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = torch.zeros(m, k, device="cuda", dtype=torch.float16), whole(g, n, k)
+    at = torch.cat([torch.arange(0, 300), torch.arange((1 << 29) - 100, (1 << 29) + 100), torch.arange(m - 300, m)]).cuda()
+    x[at] = whole(g, at.numel(), k)
+    got = L.linear(x, w)
+    assert torch.equal(got[at].double(), R.mm(x[at].double(), w.double()))
+    assert not bool(got[300:(1 << 29) - 100].any()) and not bool(got[(1 << 29) + 100:m - 300].any())
