@@ -463,9 +463,17 @@ __global__ __launch_bounds__(256) void linear_gate_kernel(const LinearGateParams
 // partial sums [blocks][pitch] to dst[n], pitch a multiple of 16
 template <class T>
 __global__ __launch_bounds__(256) void rows_sum_kernel(const float *partial, int blocks, int pitch, void *dst, int n) {
-  const float total = column_final_sum(partial, pitch, 0, blocks, blockIdx.x);
-  const int c = blockIdx.x * 16 + threadIdx.x;
+  const int group = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+  if (group * 16 >= n) return;
+  const float total = column_final_sum(partial, pitch, 0, blocks, group);
+  const int c = group * 16 + threadIdx.x;
   if (threadIdx.x < 16 && c < n) reinterpret_cast<uint16_t *>(dst)[c] = Elem<T>::from_float(total);
+}
+
+// workgroups of 256 threads for `groups` of 16 columns (a launch has fewer than 2^32 threads along a side)
+dim3 rows_sum_grid(int pitch) {
+  const int64_t groups = pitch / 16, wide = std::min<int64_t>(groups, 1 << 20);
+  return dim3((unsigned)wide, (unsigned)((groups + wide - 1) / wide));
 }
 
 template <class T, bool NORM, bool CODES, int G, int P, bool LONG = false>
@@ -522,7 +530,7 @@ hipError_t norm_backward_of(const NormGradParams &p, hipStream_t s) {
   else hipLaunchKernelGGL((norm_backward_long_kernel<T, false>), grid, dim3(1024), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
-  hipLaunchKernelGGL(rows_sum_kernel<T>, dim3((unsigned)(p.pitch / 16)), dim3(256), 0, s, p.partial, p.blocks, p.pitch, p.grad_weight, p.k);
+  hipLaunchKernelGGL(rows_sum_kernel<T>, rows_sum_grid(p.pitch), dim3(256), 0, s, p.partial, p.blocks, p.pitch, p.grad_weight, p.k);
   return hipGetLastError();
 }
 
@@ -588,8 +596,8 @@ hipError_t launch_linear_gate(LinearGateParams p, int64_t dz_pitch, void *grad_b
   else stream ? launch(linear_gate_kernel<F16, true>) : launch(linear_gate_kernel<F16, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.partial == nullptr) return e;
-  if (bf16) hipLaunchKernelGGL(rows_sum_kernel<BF16>, dim3((unsigned)(p.pitch / 16)), dim3(256), 0, s, p.partial, blocks, p.pitch, grad_bias, p.n);
-  else hipLaunchKernelGGL(rows_sum_kernel<F16>, dim3((unsigned)(p.pitch / 16)), dim3(256), 0, s, p.partial, blocks, p.pitch, grad_bias, p.n);
+  if (bf16) hipLaunchKernelGGL(rows_sum_kernel<BF16>, rows_sum_grid(p.pitch), dim3(256), 0, s, p.partial, blocks, p.pitch, grad_bias, p.n);
+  else hipLaunchKernelGGL(rows_sum_kernel<F16>, rows_sum_grid(p.pitch), dim3(256), 0, s, p.partial, blocks, p.pitch, grad_bias, p.n);
   return hipGetLastError();
 }
 

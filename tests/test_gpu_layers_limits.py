@@ -44,3 +44,22 @@ def test_linear_of_very_many_rows(L):
     got = L.linear(x, w)
     assert torch.equal(got[at].double(), R.mm(x[at].double(), w.double()))
     assert not bool(got[300:(1 << 29) - 100].any()) and not bool(got[(1 << 29) + 100:m - 300].any())
+
+
+@pytest.mark.parametrize("k", [(1 << 28) + 24, (1 << 24) + 17])
+def test_norm_of_one_very_long_row(L, k):
+    """Elements of +-1 and +-2 in a row: the statistics are those of their counts."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    signs = lambda: (torch.randint(0, 2, (1, k), generator=g, device="cuda", dtype=torch.int8) * 2 - 1).half()
+    x, w, dy = signs() * 2, torch.ones(k, device="cuda", dtype=torch.float16), signs()
+    leaves = [t.requires_grad_() for t in (x, w)]
+    out = L.rms_norm(*leaves, 1e-6)
+    gx, gw = torch.autograd.grad(out, leaves, dy)
+    with torch.no_grad():
+        assert torch.equal(out, x / 2) and torch.equal(gw, (x / 2 * dy)[0])
+        # u = x / 2, grad_x = (dy - u mean(dy u)) / 2: the mean, of a sum in 32 bits of k terms, is off by no more than k 2^-24; one rounding
+        mean = float((dy * (x / 2)).double().mean())
+        want = (dy.float() - x / 2 * mean) / 2
+        # sums of a thread's share, then of the threads': k / 1024 + 1024 additions
+        allowed = (k / 1024 + 1024) * 2.0 ** -24 / 2 + 2.0 ** -12
+        assert float((gx.float() - want).abs().max()) <= allowed
