@@ -52,9 +52,9 @@ __device__ __forceinline__ void row_sum_max(float &sum, float &top, float2 *lds)
   }
 }
 
-// The whole number next to 127 v / top.  q = v * (127 / top) in 32 bits is within 2^-16 of it (three roundings of at most
-// 2^-24 of 127); where a tie may be that near, the two sides of the tie are compared exactly: 254 |v| against (2 n + 1) top, each
-// a product of 24 by 9 bits.
+// The whole number next to 127 v / top.  q = v * (127 / top) in 32 bits is within 1.52e-5 of it: two roundings, of the quotient and of the
+// product, of at most 2^-24 of 127 each (the lift below is a power of two).  Where a tie is nearer than twice that, the two sides of the
+// tie are compared exactly: 254 |v| against (2 n + 1) top, each a product of 24 by 9 bits.
 __device__ __forceinline__ int code_of(float v, float inv, double top) {
   const float q = v * inv, r = __builtin_rintf(q);
   int code = (int)r;
