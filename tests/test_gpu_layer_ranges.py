@@ -77,3 +77,28 @@ def test_infinite_gradients_stop_at_a_gate(L, monkeypatch, act, n, residual, pyt
     assert torch.equal(gx[rows, 1], (passes[rows] * n * 2.0 ** -9).half())
     assert float(gx[4, 1]) == math.inf and float(gx[3, 1]) == (0 if act == "relu" else math.inf)
     assert float(gb[6]) == math.inf and (act == "leaky_relu" or bool(gb[5].isfinite()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [64, 136])
+def test_the_lower_tail_of_a_gelu(L, dtype, n):
+    """Relative to the value, down to where bf16 ends: the result, and the slope by the gradient of x."""
+    eps, tiny = {torch.float16: (2.0 ** -11, 2.0 ** -25), torch.bfloat16: (2.0 ** -8, 2.0 ** -134)}[dtype]
+    z = -torch.linspace(0.5, 12.5, 3000, device="cuda").to(dtype).unique().flip(0)
+    x, w = torch.zeros(z.numel(), 8, device="cuda", dtype=dtype), torch.zeros(n, 8, device="cuda", dtype=dtype)
+    x[:, 0], w[0, 0] = z, 1      # (one channel is the argument, the others' is zero)
+    dy = torch.zeros(z.numel(), n, device="cuda", dtype=dtype)
+    dy[:, 0] = 1
+    leaves = [t.requires_grad_() for t in (x, w)]
+    out = L.linear(*leaves, activation="gelu")
+    gx, = torch.autograd.grad(out, [x], dy)
+    d = z.double()
+    # the tail's quotient 1.6e-4 and its evaluation 2^-18; the exponent, of up to 113, is off by two roundings of 2^-24, times ln 2
+    off = 1.7e-4 + 2.0 ** -18 + 113 * 2.0 ** -23 * 0.7
+    want = d * 0.5 * torch.special.erfc(-d / math.sqrt(2))
+    assert ((out[:, 0].double() - want).abs() <= want.abs() * (eps + off) * 1.01 + tiny).all()
+    # the slope is tail + z density, of opposite signs: errors of both count; dz and grad_x are rounded
+    density = torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
+    slope = want / d + d * density
+    allowed = (want / d * off + d.abs() * density * off) * 1.01
+    assert ((gx[:, 0].double() - slope).abs() <= allowed + (slope.abs() * eps + tiny) * 2.02).all()
