@@ -10,6 +10,12 @@ namespace cummhip {
 #define CUMM_CAT_(a, b) a##b
 #define CUMM_CAT(a, b) CUMM_CAT_(a, b)
 
+// Up to 16 rows: two waves a workgroup from more columns on than one workgroup per CU takes, else eight.  us with two and with eight, one row,
+// bf16, weights that no cache holds, k 256, 1024, 4096, 8192: 2048 columns 3.2 4.0 7.6 15.3 and 3.5 3.9 7.0 11.6, 4096 3.4 4.1 10.7 18.9 and 3.6 4.7 9.2 17.7,
+// 6144 3.8 5.0 12.3 24.3 and 5.3 7.3 14.2 25.9, 8192 3.9 5.3 15.3 32.5 and 5.6 7.7 16.6 31.7, 28672 7.9 14.2 45.4 94.9 and 16.5 22.9 46.4 92.9; 16 rows and
+// 8-bit operands within 5 % of the same.
+constexpr int kFewWide = 4096;
+
 #ifdef CUMM_LINEAR_HOST
 
 // Which kernel and how many slices: the least estimated time, in us on 256 CUs.  The figures are fitted (non-negative least
@@ -18,6 +24,7 @@ namespace cummhip {
 // slices tried, on 1870 other products (fitted to those 4.2 %, but then 392 x 568 over 42200 rows takes 99 us
 // instead of 46).  R: workgroups per CU, rounded up while there are one or two (one per CU: always), as they are beyond; steps of 64 k.
 //   launch + R (turn + step * steps) + MB of operands and result + MB of partial sums + joining them, by R = 1, 2, more
+// f16 and 8-bit operands take the same figures (k of those in pairs): 4.0 and 5.2 % slower than the fastest on 300 other forward products each.
 // 64 x 64 in four waves and two stages (rows by the hundred thousand and a step or two: 119985 x 64 x 64 9.5 us against 12.7),
 // or in 2 x 2 x 2 waves and three; 64 x 128 in 2 x 4, three stages; both with steps of 128 k where a CU has one workgroup; the others
 // through registers.  Few rows (17 to 64; up to 16 always): 16 columns per workgroup.  What decides: up to 32 rows nearly always the kernel for few
@@ -76,7 +83,7 @@ LinearPlan linear_plan(LinearLayout layout, int64_t m, int n_, int64_t k) {
 bool linear_plan_fits(const LinearPlan &plan, int64_t m, int n) {
   const auto threads = [&](int64_t tm, int64_t tn, int64_t per) { return (m + tm - 1) / tm * ((n + tn - 1) / tn) * per < (int64_t)1 << 32; };
   switch (plan.tile) {
-  case kTileFew: return threads(m, 16, m > 16 ? 256 : (n >= 8192 ? 128 : 512));
+  case kTileFew: return threads(m, 16, m > 16 ? 256 : (n > kFewWide ? 128 : 512));
   case kTile64Small: return threads(64, 64, 256);
   case kTile64: return threads(64, 64, 512);
   case kTile64x128: return threads(64, 128, 512);
@@ -171,9 +178,7 @@ static hipError_t launch_layout(const LinearPlan &plan, const LinearParams &p, h
   switch (plan.tile) {
   case kTileFew:
     if constexpr (!XT && !YT) {
-      // (two waves where there are several workgroups per CU, else eight: 1 x 4096 x 16384 bf16 26.9 us against 28.5,
-      // 4 x 8192 x 256 13.8 against 6.7)
-      if (p.m <= 16) return p.n >= 8192 ? few<T, OUT, 2, 1, 2, 4>(p, s) : few<T, OUT, 8, 1, 2, 3>(p, s);
+      if (p.m <= 16) return p.n > kFewWide ? few<T, OUT, 2, 1, 2, 4>(p, s) : few<T, OUT, 8, 1, 2, 3>(p, s);
       if (p.m <= 32) return few<T, OUT, 4, 2, 2, 3>(p, s);
       if (p.m <= 64) return few<T, OUT, 4, 4, 2, 3>(p, s);
     }

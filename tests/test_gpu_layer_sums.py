@@ -56,3 +56,18 @@ def test_rms_norm_loses_no_row(L, residual, dtype, m, k):
         if residual:
             want = want + ds.float()
         assert torch.equal(gx, want.to(dtype))
+
+
+@pytest.mark.parametrize("m", [1, 7, 16])
+@pytest.mark.parametrize("k,n", [(64, 4096), (64, 4104), (1000, 5001), (520, 8184), (4096, 8200)])
+@pytest.mark.parametrize("dtype", HALVES + [torch.int8])
+def test_few_rows_of_many_columns(L, dtype, m, k, n):
+    """Both kernels for few rows, on either side of the line between them."""
+    x, w, b, r, _ = W.linear(m, k, n, "cuda")
+    want = torch.mm(x.float(), w.float().t().contiguous()) + b.float() + r.float()
+    if dtype == torch.int8:
+        one = lambda c: torch.ones(c, device="cuda")
+        got = L.linear_s8(x, one(m), w, one(n), b.float(), residual=r.half(), dtype=torch.float16)
+    else:
+        got = L.linear(x.to(dtype), w.to(dtype), b.to(dtype), residual=r.to(dtype))
+    assert torch.equal(got, want.to(got.dtype))
