@@ -11,7 +11,8 @@ bool simple(const Tensor &t, const c10::Device &device, at::ScalarType type) {
          !t.key_set().has(c10::DispatchKey::Python) && !t._fw_grad(0).defined();
 }
 
-// A tensor's rows: the tensor itself, or a contiguous copy where its rows are not contiguous and evenly apart
+// A tensor's rows: the tensor itself, or a contiguous copy where its rows are not contiguous and evenly apart, or further apart than
+// a product takes them (8 MiB)
 struct Rows {
   Tensor t;
   int64_t rows = 0, cols = 0, pitch = 0;
@@ -22,7 +23,7 @@ struct Rows {
     pitch = cols;
     if (t.is_contiguous()) return;
     if (t.dim() != 2) t = t.reshape({-1, cols});      // (a view where the rows are evenly apart)
-    if (t.dim() == 2 && (t.stride(1) == 1 || cols == 1) && (rows == 1 || t.stride(0) >= cols)) {
+    if (t.dim() == 2 && (t.stride(1) == 1 || cols == 1) && (rows == 1 || (t.stride(0) >= cols && t.stride(0) * (int64_t)t.element_size() < (int64_t)8 << 20))) {
       if (rows > 1) pitch = t.stride(0);
       return;
     }

@@ -67,10 +67,11 @@ def _made(fn, *args):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as a matrix of its rows, without a copy where the rows are contiguous and evenly apart."""
+    """``t`` as a matrix of its rows, without a copy where the rows are contiguous and evenly apart, by less than the 8 MiB that
+    a product takes."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    if t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < (8 << 20) // t.element_size():
         t = t.contiguous()
     return t
 

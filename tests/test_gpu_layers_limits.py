@@ -63,3 +63,25 @@ def test_norm_of_one_very_long_row(L, k):
         # sums of a thread's share, then of the threads': k / 1024 + 1024 additions
         allowed = (k / 1024 + 1024) * 2.0 ** -24 / 2 + 2.0 ** -12
         assert float((gx.float() - want).abs().max()) <= allowed
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_rows_very_far_apart(L, monkeypatch, python):
+    """Columns of a matrix whose rows are 8 MiB and more: copied, for the gradient of the result too."""
+    if python:
+        from cumm_amd import torch_bridge
+        monkeypatch.setattr(torch_bridge, "_native_module", False)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for columns in ((4 << 20) - 1, 4 << 20, 5 << 20):
+        wide = torch.zeros(6, columns, device="cuda", dtype=torch.float16)
+        wide[:, 8:280] = whole(g, 6, 272)
+        for n in (64, 136):
+            w, norm = whole(g, n, 136), whole(g, 136)
+            x, dy, r = wide[:, 8:144], wide[:, 144:144 + n], wide[:, 140:140 + n]
+            near = [t.contiguous() for t in (x, dy, r)]
+            for act in ("none", "relu"):
+                step = lambda x, dy, r: (L.linear(x, w, activation=act, residual=r),) + torch.autograd.grad(
+                    L.linear(x.requires_grad_(), w.requires_grad_(), activation=act, residual=r), (x, w), dy)
+                assert all(torch.equal(a, b) for a, b in zip(step(x.detach(), dy, r), step(near[0].detach(), *near[1:])))
+            assert torch.equal(L.rms_norm(x, norm), L.rms_norm(near[0], norm))
+            assert all(torch.equal(a, b) for a, b in zip(L.quantize_rows(x), L.quantize_rows(near[0])))
