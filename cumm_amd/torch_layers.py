@@ -240,10 +240,11 @@ def _linear_args(name, x, weight, bias, residual, activation, out_dtype, bias_dt
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "none",
            residual: Optional[torch.Tensor] = None, slope: float = 0.01) -> torch.Tensor:
-    """``act(x @ weight.T + bias) + residual`` for x [..., K], weight [N, K] (f16 / bf16); one rounding.  Differentiable in
-    all four tensors (once); with N and K multiples of 8 up to 128, the backward pass works out what the activation got from x,
-    weight and bias, which are kept for that, or, for "relu" and "leaky_relu", keeps which elements pass, a bit each, decided by the
-    exact sign of the activation's argument.  ``slope`` is that of "leaky_relu"."""
+    """``act(x @ weight.T + bias) + residual`` for x [..., K], weight [N, K] (f16 / bf16); the result is rounded
+    once.  Differentiable in all four tensors (once): the gradient of what the activation got is rounded to the tensors' type
+    before its products with weight and x, and so is what the activation got where it is kept.  With N and K multiples of 8 up to
+    128 it is worked out again from x, weight and bias, which are kept for that, or, for "relu" and "leaky_relu", which elements pass is
+    kept, a bit each, decided by the exact sign of the activation's argument.  ``slope`` is that of "leaky_relu"."""
     native = _native()
     if native is not None and activation in ACTIVATIONS:
         out = native.layer_linear(x, weight, bias, residual, ACTIVATIONS[activation], slope)
