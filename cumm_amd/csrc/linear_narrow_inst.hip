@@ -49,6 +49,7 @@ __device__ __forceinline__ v4i turning_read(const char *tile, int row, int col) 
 // The error is at most (k + 8) 2^-23 of the sum of the products' magnitudes, in whatever order the matrix instructions add and
 // whether they round or cut, and that sum at most the length of x's row times that of the weight's (Cauchy-Schwarz): one
 // product and a comparison per element, and of ordinary numbers one element in 18000 (64 channels in) is that near.
+// (bf16 rows whose squares leave 32 bits: above 1e19 all of a row is added up in 64, below 1e-19 it is left to its 32-bit sums.)
 // the sum over the four lanes that share a row, lane & 15 alike (swaps of halves and quarters of a wave: no trip through LDS)
 __device__ __forceinline__ uint2 four_swap(uint32_t v, bool halves) {
   const auto r = halves ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
