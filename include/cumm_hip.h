@@ -538,9 +538,9 @@ int cumm_hip_relu_backward_sums(void *gated, void *sums, const void *grad, const
  *   pre_act, unless NULL, gets what the activation gets (rounded): the backward pass wants it.
  *   out may be residual itself, with its pitch; apart from that no output overlaps an operand.
  *   m == 0 is no work; NaN passes through every activation.
- *   ReLU and leaky ReLU of f16 / bf16 layers with n and k multiples of 8 up to CUMM_HIP_LINEAR_NARROW: an argument that 32 bits cannot
- *   tell from zero is added up in 64, so that its sign is right (of bf16 rows below 1e-19 it is that of the 32-bit sum), and gate, unless NULL (it is for these layers only, 4-byte aligned), gets
- *   which elements of the gradient pass, for the backward pass to read.
+ *   ReLU and leaky ReLU of f16 / bf16 layers with n and k multiples of 8 up to CUMM_HIP_LINEAR_NARROW: an argument that 32 bits
+ *   cannot tell from zero is added up in 64, so that its sign is right (of bf16 rows below 1e-19 it is that of the 32-bit sum), and
+ *   gate, unless NULL (it is for these layers only, 4-byte aligned), gets which elements of the gradient pass, for the backward pass.
  * cumm_hip_linear_backward: the gradients for grad_out [m, n], each NULL where it is not wanted:
  *     dz = grad_out act'(pre_act);  grad_x = dz weight [m, k];  grad_weight = dz^T x [n, k];  grad_bias = sum of dz's rows
  *   (the residual's is grad_out).  A ReLU's dz is grad_out itself or zero, that of an argument that is NaN the former; leaky likewise.
